@@ -62,6 +62,16 @@ class LayerKV:
     planes: int = 2
 
 
+@dataclass
+class SharedPrefixes:
+    """Which sequences of a step hold the same pages for a prefix, as an attention kernel wants it (int32 on the device; ``KVCache.shared_prefixes``
+    finds them).  The pages of a group are the first ones of all its sequences' tables and lie below their newest positions."""
+    order: torch.Tensor          # [seqs] the step's sequences, group by group, those of no group at any place
+    own_page: torch.Tensor       # [seqs] pages that sequence i has in common with its group (0: it is in none); its own begin there
+    groups: torch.Tensor         # [groups, 3] place of the group's first sequence in ``order``, sequences, pages
+    most: int                    # sequences of the largest group
+
+
 class KVGroup:
     def __init__(self, index: int, request: KVRequest, layers: List[int], n_pages: int, n_slots: int,
                  page_size: int, max_pages_per_seq: int, dtype: torch.dtype, device):

@@ -8,14 +8,14 @@ built or loaded, ``Kernels()`` raises.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from .csrc.build import BuildError, library_path
 
 F32, BF16 = 0, 1
-ABI_VERSION = 39
+ABI_VERSION = 40
 SPLIT_BLOCKS = 296          # blocks of the decode attention that one wave holds (two per SM, 148 SMs)
 TC_ATTENTION_MIN_LEN = 256  # prompts from this length on take the tcgen05 attention (head_dim 64 or 128)
 SPLIT_FEW_BLOCKS = 148      # below this many blocks at 8 splits, more splits are taken
@@ -117,6 +117,17 @@ def extend_splits(blocks: int, max_len: int, window: int, keep_first: int) -> in
     return max(1, min(64, tiles // 4, EXTEND_BLOCKS // max(1, blocks)))
 
 
+def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_heads: int, max_len: int) -> Tuple[int, int]:
+    """(splits of a group's prefix, splits of a sequence's own pages) of ``Kernels.attention_shared``: about one wave of blocks for each."""
+    group = n_heads // n_kv_heads
+    rows = most * group
+    tile = 16 if rows <= 16 else 32 if rows <= 32 else 64
+    pages = -(-max_len // 64) if max_len > 0 else 1 << 20
+    prefix = n_groups * -(-rows // tile) * n_kv_heads
+    own = n_seqs * n_kv_heads * -(-group // 16)
+    return (max(1, min(64, SPLIT_BLOCKS // max(1, prefix), pages)), max(1, min(32, SPLIT_BLOCKS // own, pages)))
+
+
 # epilogues of the skinny product
 SK_STORE, SK_ACCUM, SK_SWIGLU, SK_STORE_F32 = 0, 1, 2, 3
 EPI_ACT = 4                 # grouped tcgen05 product only: an ungated activation, bfloat16 store
@@ -162,6 +173,8 @@ _SIGNATURES = {
     "cima_attention_decode": [_vp, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _i, _i, _f, _i, _i, _vp, _i, _vp, _vp],
     "cima_attention_decode_near": [_vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _i, _vp],
     "cima_attention_decode_near_room": [_i, _vp],
+    "cima_attention_shared": [_vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _f, _f, _vp, _i,
+                              _vp, _i, _vp],
     "cima_attention_prefill": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _f, _i, _i, _vp, _i, _vp, _vp],
     "cima_attention_extend": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _f, _i, _i, _vp, _i, _vp,
                               _i, _vp, _vp, _vp],
@@ -211,6 +224,8 @@ _SIGNATURES = {
     "cima_branch_norm": [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _f, _vp],
     "cima_softcap": [_vp, _sz, _f, _vp],
     "cima_argmax": [_vp, _i, _i, _i, _vp, _vp],
+    "cima_token_logprobs": [_vp, _i, _i, _vp, _vp, _vp],
+    "cima_copy_pages": [_vp, _i, ctypes.c_longlong, _i, _i, ctypes.c_longlong, _vp, _i, _vp],
     "cima_sample": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "cima_sample_general": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
 }
@@ -282,6 +297,14 @@ class Kernels:
             raise KernelError(f"{name} has {t.dim()} dimensions, expected {dims}")
         if not t.is_contiguous():
             raise KernelError(f"{name} is not contiguous")
+
+    @staticmethod
+    def _here(*tensors: torch.Tensor) -> None:
+        """The tensors lie on the current device, whose stream the kernel goes to."""
+        at = torch.cuda.current_device()
+        for t in tensors:
+            if t.get_device() != at:
+                raise KernelError(f"a tensor on {t.device} while cuda:{at} is the current device")
 
     # ------------------------------------------------------------------ elementwise
     def embed(self, ids: torch.Tensor, table: torch.Tensor, x: torch.Tensor, scale: float = 1.0,
@@ -840,6 +863,61 @@ class Kernels:
             qkv.data_ptr(), qkv.shape[1], kv.storage.data_ptr(), kv.block_table.data_ptr(), kv.block_table.shape[1], kv.ring_pages,
             seq_slot.data_ptr(), seq_len.data_ptr(), out.data_ptr(), out.shape[1], B, n_heads, n_kv_heads, head_dim, scale, window, cluster,
             int(early), self._stream()), "attention_decode_near")
+
+    def attention_shared(self, qkv: torch.Tensor, kv, seq_slot, seq_len, shared, out: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
+                         scale: float, max_len: int = 0, early: bool = False, sink: float = 0.0, head_sink=None, gate_col: int = 0, slopes=None,
+                         splits: Optional[Tuple[int, int]] = None) -> None:
+        """One query per sequence over the paged cache where groups of sequences hold the same pages for a prefix (``shared``, a
+        ``SharedPrefixes``): a group's prefix is read once for all its sequences.  bfloat16 (head sizes that are multiples of 16) or float32
+        (multiples of 4) up to 128, pages of 64, every key visible; ``max_len``: positions of the longest sequence (0: not known; it bounds the
+        splits); the other arguments are ``attention_decode``'s."""
+        self._need(qkv, "qkv", None, 2); self._need(out, "out", qkv.dtype, 2)
+        self._need(kv.storage, "cache", qkv.dtype, 5); self._need(kv.block_table, "block_table", torch.int32, 2)
+        B, groups = qkv.shape[0], shared.groups
+        for n, t in (("seq_slot", seq_slot), ("seq_len", seq_len), ("order", shared.order), ("own_page", shared.own_page)):
+            self._need(t, n, torch.int32, 1)
+            if t.numel() < B:
+                raise KernelError(f"attention_shared: {n} has {t.numel()} entries for {B} sequences")
+        self._need(groups, "groups", torch.int32, 2)
+        self._here(qkv, out, kv.storage, kv.block_table, seq_slot, seq_len, shared.order, shared.own_page, groups)
+        self._need_head_sink(head_sink, n_heads, slopes)
+        if kv.ring_pages or kv.window:
+            raise KernelError("attention_shared: a layer with a window keeps no prefix to share")
+        if tuple(out.shape) != (B, n_heads * head_dim) or tuple(kv.storage.shape[1:]) != (kv.planes, n_kv_heads, kv.page_size, head_dim):
+            raise KernelError(f"attention_shared: out {tuple(out.shape)} or cache pages {tuple(kv.storage.shape)} do not fit {B} rows of {n_heads} heads of {head_dim}")
+        if groups.shape[1] != 3 or qkv.shape[1] < n_heads * head_dim:
+            raise KernelError(f"attention_shared: groups {tuple(groups.shape)} are not [groups, 3], or rows of {qkv.shape[1]} hold no {n_heads} heads of {head_dim}")
+        n_groups, most = groups.shape[0], shared.most
+        np_, no = splits or shared_splits(n_groups, most, B, n_heads, n_kv_heads, max_len)
+        if not self._admit(f"attention_shared[{np_} + {no} splits]", *self._attention_work(qkv, n_heads, n_kv_heads, head_dim, kv.planes)): return
+        # this call's own, as attention_decode's
+        cells = B * n_heads * (np_ + no)
+        part = torch.empty(cells * (head_dim + 2), dtype=torch.float32, device=qkv.device)
+        at = part.data_ptr()
+        self._check(self.lib.cima_attention_shared(
+            qkv.data_ptr(), dtype_code(qkv.dtype), qkv.shape[1], kv.storage.data_ptr(), kv.block_table.data_ptr(), kv.block_table.shape[1], kv.page_size,
+            kv.planes, seq_slot.data_ptr(), seq_len.data_ptr(), shared.order.data_ptr(), shared.own_page.data_ptr(), groups.data_ptr(), n_groups, most,
+            at, at + 4 * cells * head_dim, np_, no, out.data_ptr(), out.shape[1], B, n_heads, n_kv_heads, head_dim, scale, sink, _ptr(head_sink),
+            gate_col, _ptr(slopes), int(early), self._stream()), "attention_shared")
+        self.launches += 1
+
+    # ------------------------------------------------------------------ pages
+    def copy_pages(self, storage: torch.Tensor, plan: torch.Tensor) -> None:
+        """storage[:, to, :, :, :n] = storage[:, from, :, :, :n] for each (from, to, n) of ``plan`` (int32 [entries, 3] on the host), in one launch
+        for up to 320 entries.  ``storage`` [layers, pages, planes, heads, positions, values], any element type of 2 bytes or more (bits are
+        moved).  No page may be written twice, or both read and written: the copies have no order among them."""
+        self._need(storage, "storage", None, 6)
+        self._here(storage)
+        if plan.is_cuda or plan.dtype is not torch.int32 or plan.dim() != 2 or plan.shape[1] != 3 or not plan.is_contiguous():
+            raise KernelError(f"copy_pages: the plan {tuple(plan.shape)} {plan.dtype} on {plan.device} is not int32 [entries, 3] on the host")
+        layers, pages, planes, heads, size, values = storage.shape
+        row = values * storage.element_size()
+        n = plan.shape[0]
+        if n == 0 or storage.numel() == 0:
+            return
+        if not self._admit("copy_pages", 2.0 * layers * planes * heads * row * float(plan[:, 2].sum()) if self.profile is not None else 0): return
+        self._check(self.lib.cima_copy_pages(storage.data_ptr(), layers, pages, planes * heads, size, row, plan.data_ptr(), n, self._stream()), "copy_pages")
+        self.launches += (n - 1) // 320
 
     # ------------------------------------------------------------------ short convolution, depth average, latents
     def short_conv(self, h: torch.Tensor, w: torch.Tensor, state: Optional[torch.Tensor], batch, out: torch.Tensor,
@@ -1718,6 +1796,17 @@ class Kernels:
             raise KernelError(f"argmax: {tokens.numel()} token places for {n} rows")
         if not self._admit("argmax", n * V * 4): return
         self._check(self.lib.cima_argmax(logits.data_ptr(), V, n, V, tokens.data_ptr(), self._stream()), "argmax")
+
+    def token_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, out: torch.Tensor) -> None:
+        """out[i] = log softmax(logits[i])[tokens[i]] in float32.  A row with a NaN or +inf, or of nothing but -inf, gives NaN, and so does a token
+        outside the vocabulary."""
+        self._need(logits, "logits", torch.float32, 2); self._need(tokens, "tokens", torch.int32, 1); self._need(out, "out", torch.float32, 1)
+        self._here(logits, tokens, out)
+        n, V = logits.shape
+        if tokens.numel() != n or out.numel() != n:
+            raise KernelError(f"token_logprobs: {tokens.numel()} tokens and {out.numel()} places for {n} rows")
+        if not self._admit("token_logprobs", n * V * 4): return
+        self._check(self.lib.cima_token_logprobs(logits.data_ptr(), n, V, tokens.data_ptr(), out.data_ptr(), self._stream()), "token_logprobs")
 
     def sample(self, logits: torch.Tensor, row_slot: torch.Tensor, params: torch.Tensor, rng: torch.Tensor,
                ring: torch.Tensor, count: torch.Tensor, work: torch.Tensor, tokens: torch.Tensor,

@@ -1,0 +1,253 @@
+"""Attention over shared prefixes, copies of pages and log-probabilities of tokens against plain implementations in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from shared_cases import PAGE, logprob_reference, shared_case, shared_reference
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def K():
+    from cima_b200.kernels import Kernels
+    return Kernels(verbose=False)
+
+
+def run_shared(K, c, splits=None, **more):
+    from cima_b200.cache import LayerKV, SharedPrefixes
+    kv = LayerKV(c.storage, c.table, PAGE, 0, 0, 0, c.planes)
+    out = torch.full((c.B, c.heads * c.hd), 7.0, dtype=c.dtype, device=c.qkv.device)
+    K.attention_shared(c.qkv, kv, c.slot, c.len, SharedPrefixes(c.order, c.own_page, c.groups, c.most), out, c.heads, c.kv_heads, c.hd, c.scale,
+                       c.max_len, splits=splits, **more)
+    return out
+
+
+def check(got, want, tol):
+    off = (got.double().cpu() - want).abs()
+    assert torch.isfinite(got.float()).all()
+    assert (off <= tol).all(), f"{int((off > tol).sum())} values, worst {float((off / tol).max()):.3g} times the bound"
+
+
+SIZES = [
+    # counts, prefix pages, own positions, alone, heads, kv, hd
+    ([2], [1], [1], [], 1, 1, 64),
+    ([2], [5], [1, 40], [], 14, 2, 64),
+    ([8], [32], [1, 63, 64, 65, 100], [], 28, 4, 128),
+    ([3], [3], [17], [1, 64, 700], 4, 2, 16),
+    ([2, 5, 9], [1, 4, 2], [1, 2, 130, 64], [5], 12, 2, 128),
+    ([19], [3], [33, 1], [], 40, 8, 128),
+    ([70], [9], [1, 200, 64], [], 28, 4, 128),
+    ([33], [7], [5, 64], [900], 40, 2, 64),
+    ([2, 2], [2, 6], [300, 9], [], 6, 3, 48),
+    ([4], [2], [77], [3], 8, 2, 112),
+    ([4], [2], [77], [3], 5, 1, 96),
+    ([], [], [], [1, 65, 128], 8, 2, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("planes", [2, 1])
+@pytest.mark.parametrize("size", SIZES, ids=[str(i) for i in range(len(SIZES))])
+def test_shared_attention(K, size, planes, dtype):
+    counts, prefix, own, alone, heads, kv, hd = size
+    c = shared_case(counts, prefix, own, heads, kv, hd, dtype, planes=planes, alone=alone, seed=len(counts) + heads)
+    check(run_shared(K, c), *shared_reference(c))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("what", ["sink", "head_sink", "slopes", "gate", "all"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_shared_attention_forms(K, what, dtype, hd):
+    c = shared_case([6, 2], [3, 1], [1, 64, 90], 14, 2, hd, dtype, alone=[70], gate=what in ("gate", "all"), seed=11)
+    more = {}
+    if what == "sink":
+        more["sink"] = 2.0
+    if what in ("head_sink", "all"):
+        more["head_sink"] = c.sink
+    if what in ("slopes", "all"):
+        more["slopes"] = c.slopes
+    if what in ("gate", "all"):
+        more["gate_col"] = c.gate_col
+    check(run_shared(K, c, **more), *shared_reference(c, **more))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("splits", [(1, 1), (3, 2), (64, 32), (64, 64), (1, 127)])
+def test_shared_attention_splits(K, splits, dtype):
+    c = shared_case([5], [11], [1, 64, 150], 12, 2, 64, dtype, alone=[1, 500], seed=3)
+    check(run_shared(K, c, splits=splits), *shared_reference(c))
+
+
+def test_shared_attention_large_scores(K):
+    """Scores of several hundred, of both signs: the parts' maxima lie far from one another and a part's weight may vanish."""
+    c = shared_case([4], [4], [70, 3], 8, 2, 64, torch.float32, seed=9)
+    c.storage[:, 0] *= 30.0
+    check(run_shared(K, c), *shared_reference(c))
+
+
+def test_padded_groups_and_their_order(K):
+    """Groups without sequences (a recorded step's spare places) take no part; the result does not depend on which spare places there are."""
+    c = shared_case([3, 4], [2, 3], [1, 65], 14, 2, 64, torch.bfloat16, seed=5)
+    want = run_shared(K, c, splits=(4, 2))
+    c.groups = torch.cat([c.groups, torch.zeros(3, 3, dtype=torch.int32, device="cuda")])
+    assert torch.equal(run_shared(K, c, splits=(4, 2)), want)
+
+
+def test_shared_equals_unshared(K):
+    """The same batch without its groups (each sequence reads all its pages itself): within twice the bound of each other."""
+    c = shared_case([6], [9], [1, 64, 90], 28, 4, 128, torch.bfloat16, alone=[30], seed=6)
+    want, tol = shared_reference(c)
+    a = run_shared(K, c)
+    c.groups, c.own_page, c.most = c.groups[:0], torch.zeros_like(c.own_page), 0
+    check(run_shared(K, c), a.double().cpu(), 2 * tol)
+
+
+def test_shared_attention_replayed_and_on_a_stream(K):
+    c = shared_case([7], [6], [1, 64, 90], 14, 2, 64, torch.bfloat16, seed=8)
+    want = run_shared(K, c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run_shared(K, c)
+    side.synchronize()
+    assert torch.equal(other, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run_shared(K, c)
+    for _ in range(2):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    # what a replay reads on the device may change: shorter sequences, other groups
+    c2 = shared_case([7], [6], [2, 11, 65], 14, 2, 64, torch.bfloat16, seed=21)
+    for n in ("qkv", "slot", "len", "order", "own_page", "groups"):
+        getattr(c, n).copy_(getattr(c2, n))
+    assert c.storage.shape[0] >= c2.storage.shape[0]
+    c.storage[:c2.storage.shape[0]].copy_(c2.storage)
+    c.table[:, :c2.table.shape[1]].copy_(c2.table)
+    g.replay()
+    check(out, *shared_reference(c2))
+
+
+def test_shared_attention_refusals(K):
+    from cima_b200.cache import LayerKV, SharedPrefixes
+    from cima_b200.kernels import KernelError
+    c = shared_case([2], [1], [1], 4, 2, 64, torch.bfloat16)
+    plan = SharedPrefixes(c.order, c.own_page, c.groups, c.most)
+    out = torch.empty(c.B, 256, dtype=torch.bfloat16, device="cuda")
+
+    def call(kv=None, shared=plan, out=out, heads=4, slot=c.slot, splits=None, qkv=c.qkv, **more):
+        K.attention_shared(qkv, kv or LayerKV(c.storage, c.table, PAGE, 0, 0, 0), slot, c.len, shared, out, heads, 2, 64, 0.125, splits=splits, **more)
+
+    for kw, word in [(dict(out=out[:, :128].contiguous()), "do not fit"), (dict(kv=LayerKV(c.storage, c.table, PAGE, 3, 128, 0)), "window"),
+                     (dict(slot=c.slot.long()), "expected"), (dict(slot=c.slot[:1]), "entries"), (dict(splits=(0, 1)), "splits"), (dict(splits=(64, 65)), "splits"),
+                     (dict(shared=SharedPrefixes(c.order, c.own_page, c.groups, 5)), "groups"), (dict(gate_col=c.qkv.shape[1] - 8), "gate"),
+                     (dict(shared=SharedPrefixes(c.order.cpu(), c.own_page, c.groups, 2)), "GPU tensors"), (dict(heads=3, out=out[:, :192].contiguous()), "multiple"),
+                     (dict(kv=LayerKV(c.storage.half(), c.table, PAGE, 0, 0, 0)), "expected"), (dict(slopes=c.slopes[:2]), "slopes"),
+                     (dict(shared=SharedPrefixes(c.order, c.own_page, c.groups[:, :2].contiguous(), 2)), "groups")]:
+        with pytest.raises(KernelError, match=word):
+            call(**kw)
+    call()
+
+
+# ---------------------------------------------------------------------------------------------- pages
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 9, 1, 1, 64, 16), (3, 40, 2, 4, 64, 128), (24, 700, 2, 2, 64, 8), (1, 6, 1, 1, 1, 1), (2, 7, 1, 3, 16, 3), (1, 30, 1, 1, 1, 500)])
+def test_copy_pages(K, shape, dtype):
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randint(-1 << 14, 1 << 14, shape, generator=gen)
+    x = x.to(dtype) if dtype.is_floating_point or dtype is torch.int64 else x.to(dtype)
+    n = (shape[1] - 1) // 2
+    ids = torch.randperm(shape[1], generator=gen)
+    fill = torch.randint(0, shape[4] + 1, (n,), generator=gen)
+    fill[0] = shape[4]
+    plan = torch.stack([ids[:n], ids[n:2 * n], fill], 1).int()
+    plan[n // 2:, 0] = plan[0, 0]                         # one page for several others
+    want = x.clone()
+    for a, b, k in plan.tolist():
+        want[:, b, :, :, :k] = x[:, a, :, :, :k]
+    got = x.cuda()
+    K.copy_pages(got, plan)
+    assert torch.equal(got.cpu(), want)
+    K.copy_pages(got, plan[:0])
+    assert torch.equal(got.cpu(), want)
+
+
+def test_copy_pages_of_a_large_storage(K):
+    """Offsets beyond 2^32 bytes and 2^31 elements."""
+    x = torch.zeros(2, 1200, 2, 8, PAGE, 1024, dtype=torch.int16, device="cuda")
+    assert x.numel() > 2 ** 31
+    x[1, 1199] = 5
+    K.copy_pages(x, torch.tensor([[1199, 1198, 33], [1199, 0, 64]], dtype=torch.int32))
+    assert (x[1, 1198, :, :, :33] == 5).all() and (x[1, 1198, :, :, 33:] == 0).all() and (x[1, 0] == 5).all() and (x[0] == 0).all() and (x[1, 1:1198] == 0).all()
+
+
+def test_copy_pages_replayed(K):
+    x = torch.randn(2, 8, 2, 2, PAGE, 16, device="cuda")
+    plan = torch.tensor([[0, 5, 20], [1, 6, 64]], dtype=torch.int32)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        K.copy_pages(x, plan)
+    plan.zero_()                                          # the recording keeps its own plan
+    x[:, 0], x[:, 1] = 3.0, 4.0
+    g.replay()
+    assert (x[:, 5, :, :, :20] == 3).all() and (x[:, 6] == 4).all() and not (x[:, 5, :, :, 20:] == 3).any()
+
+
+def test_copy_pages_refusals(K):
+    from cima_b200.kernels import KernelError
+    x = torch.zeros(1, 4, 1, 1, 4, 8, device="cuda")
+    p = lambda *rows: torch.tensor(rows, dtype=torch.int32).view(-1, 3)       # noqa: E731
+    for plan, word in [(p([0, 4, 1]), "outside"), (p([-1, 1, 1]), "outside"), (p([0, 1, 5]), "positions"), (p([0, 1, -1]), "positions"),
+                       (p([0, 1, 1], [2, 1, 1]), "writes"), (p([0, 1, 1], [1, 2, 1]), "reads"), (p([1, 2, 1], [0, 1, 1]), "writes"), (p([3, 3, 1]), "reads"),
+                       (p([0, 1, 1]).cuda(), "host"), (p([0, 1, 1]).long(), "int32")]:
+        with pytest.raises(KernelError, match=word):
+            K.copy_pages(x, plan)
+    with pytest.raises(KernelError, match="contiguous"):
+        K.copy_pages(x.transpose(1, 5), p([0, 1, 1]))
+    with pytest.raises(KernelError, match="aligned"):
+        K.copy_pages(torch.zeros(1, 4, 1, 1, 4, 8, dtype=torch.int8, device="cuda")[..., :1].contiguous(), p([0, 1, 1]))
+
+
+# ---------------------------------------------------------------------------------------------- log-probabilities
+@pytest.mark.parametrize("n, V", [(1, 1), (1, 2), (3, 7), (1, 512), (5, 1000), (2, 4097), (64, 32003), (1, 151936), (61, 152064), (700, 5001), (66000, 5)])
+@pytest.mark.parametrize("spread", [0.0, 3.0, 80.0])
+def test_token_logprobs(K, n, V, spread):
+    gen = torch.Generator(device="cuda").manual_seed(n + V)
+    x = torch.randn(n, V, generator=gen, device="cuda") * spread + 5.0
+    t = torch.randint(0, V, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    t[::2] = x[::2].argmax(1).int()
+    out = torch.full((n,), 9.0, device="cuda")
+    K.token_logprobs(x, t, out)
+    want, tol = logprob_reference(x, t)
+    off = (out.double() - want).abs()
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+def test_token_logprobs_of_infinite_logits(K):
+    inf, nan = math.inf, math.nan
+    rows = [([0.0, -inf, 1.0], 0, math.log(1 / (1 + math.e))), ([0.0, -inf, 1.0], 1, -inf), ([-inf, -inf, -inf], 1, nan), ([0.0, inf, 1.0], 0, nan),
+            ([0.0, inf, 1.0], 1, nan), ([0.0, nan, 1.0], 0, nan), ([nan, nan, nan], 2, nan), ([0.0, 0.0, 0.0], 3, nan), ([0.0, 0.0, 0.0], -1, nan),
+            ([3e38, -3e38, 0.0], 0, 0.0), ([3e38, -3e38, 3e38], 0, -math.log(2.0)), ([-inf, 4.0, -inf], 1, 0.0)]
+    x = torch.tensor([r[0] for r in rows], device="cuda")
+    t = torch.tensor([r[1] for r in rows], dtype=torch.int32, device="cuda")
+    out = torch.empty(len(rows), device="cuda")
+    K.token_logprobs(x, t, out)
+    for got, (_, _, want) in zip(out.tolist(), rows):
+        if math.isnan(want):
+            assert math.isnan(got)
+        else:
+            assert got == want or abs(got - want) <= 2.0 ** -21 * abs(want)
+
+
+def test_token_logprobs_refusals(K):
+    from cima_b200.kernels import KernelError
+    x, t, o = torch.zeros(3, 5, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"), torch.empty(3, device="cuda")
+    for args, word in [((x, t[:2], o), "tokens"), ((x, t, o[:2]), "places"), ((x.bfloat16(), t, o), "expected"), ((x, t.long(), o), "expected"),
+                       ((x.t(), t, o), "contiguous"), ((x.cpu(), t, o), "GPU")]:
+        with pytest.raises(KernelError, match=word):
+            K.token_logprobs(*args)
+    K.token_logprobs(x[:0], t[:0], o[:0])
