@@ -70,11 +70,14 @@ class LM:
         return self.model.step(entries, record=self._record)
 
     def generate(self, prompts: Sequence[Sequence[int]], options: Union[GenOptions, Sequence[GenOptions], None] = None,
-                 on_token=None, **named):
+                 on_token=None, continuations: int = 1, logprobs: bool = False, **named):
         """Token ids in, ``GenResult`` per prompt out.  Options by the reference's names
         (temperature, top_k, top_p, repeat_penalty, seed, max_tokens, stop, ignore_eos), either as a
         ``GenOptions`` (one for all prompts or one per prompt) or as keyword arguments.  ``on_token(i, token)`` is
-        called for every token of prompt ``i`` as soon as its step is read."""
+        called for every token of prompt ``i`` as soon as its step is read.
+        ``continuations`` n: n answers to each prompt, drawn with seeds that follow the option's (the first is what one answer would be); result and
+        request ``i * n + k`` is the k-th of prompt ``i``.  A prompt runs once for all its answers, which share its part of the cache.
+        ``logprobs``: each result holds its tokens' log-probabilities (``logprobs``, ``logprob``) under the model's own distribution."""
         if named:
             if options is not None and not isinstance(options, GenOptions):
                 raise ValueError("keyword options go with at most one GenOptions")
@@ -86,7 +89,37 @@ class LM:
                 else:
                     o = o.set(k, v)
             options = o
-        return self.loop.generate(prompts, options, on_token=on_token)
+        return self.loop.generate(prompts, options, on_token=on_token, continuations=continuations, logprobs=logprobs)
+
+    def score(self, sequences: Sequence[Sequence[int]], rows: int = 256) -> List[List[float]]:
+        """For each sequence of token ids the log-probability of every token but the first, given those before it.  ``rows``: the most
+        logits held at a time (a sequence runs in pieces of that many tokens)."""
+        import torch
+        from .engine import StepEntry
+        cache, kernels = self.model.cache, self.model.rt.kernels
+        if rows < 1:
+            raise ValueError(f"pieces of {rows} tokens: at least one")
+        out: List[List[float]] = []
+        for seq in sequences:
+            seq = [int(t) for t in seq]
+            if not seq:
+                raise ValueError("a sequence to score needs at least one token")
+            if min(seq) < 0 or max(seq) >= self.spec.vocab:
+                raise ValueError(f"token ids must lie in [0, {self.spec.vocab})")
+            parts = []
+            self.stepper.make_room([len(seq)], [None])
+            slots = self.stepper.open(1)
+            try:
+                for lo in range(0, len(seq) - 1, rows):
+                    piece = seq[lo:min(lo + rows, len(seq) - 1)]
+                    logits = self.model.step([StepEntry(slots[0], piece, list(range(len(piece))))], record=False)
+                    lp = torch.empty(len(piece), dtype=torch.float32, device=logits.device)
+                    kernels.token_logprobs(logits, torch.tensor(seq[lo + 1:lo + 1 + len(piece)], dtype=torch.int32, device=logits.device), lp)
+                    parts.append(lp)
+                out.append(torch.cat(parts).tolist() if parts else [])
+            finally:
+                cache.close(slots)
+        return out
 
     @property
     def stats(self):

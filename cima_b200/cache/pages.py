@@ -2,7 +2,8 @@
 
 A *slot* is a live sequence's row (of the block tables, of the length table, of
 the per-sequence state).  A *page* holds ``page_size`` consecutive positions of
-one sequence for every layer of one group.  Both allocators refuse to give out
+one sequence for every layer of one group (or of several sequences, which then
+hold it together: ``kv.py`` counts them).  Both allocators refuse to give out
 what is held and to take back what is free, so that a slot or page is never
 lost, held twice or freed twice.
 """
@@ -60,6 +61,18 @@ class FreeList:
         # keep lowest-first order of hand-out
         self._free.extend(ids)
         self._free.sort(reverse=True)
+
+    def move(self, pairs) -> None:
+        """Held ids change places with free ones: for each (old, new) the old one is free from now on and the new one held."""
+        pairs = list(pairs)
+        for old, new in pairs:
+            if not self.is_held(old) or not (0 <= new < self.n) or self._held[new]:
+                raise ValueError(f"{self.what} {old} cannot become {new}: the one must be held and the other free")
+        if len({i for p in pairs for i in p}) != 2 * len(pairs):
+            raise ValueError(f"a {self.what} moves twice in one call: {pairs}")
+        for old, new in pairs:
+            self._held[old], self._held[new] = False, True
+        self._free = [i for i in range(self.n - 1, -1, -1) if not self._held[i]]
 
     def check(self) -> None:
         """Every id is either free once or held, never both, never neither."""

@@ -1,6 +1,6 @@
 """Command line in the manner of the reference's ``cima`` (src/main.rs:19-70, :220-270):
 
-    cima run <MODEL_DIR> [TOKEN_ID ...] [--prompts FILE] [--dtype D] [--max-seq N] [--PARAM VALUE]...
+    cima run <MODEL_DIR> [TOKEN_ID ...] [--prompts FILE] [--dtype D] [--max-seq N] [--continuations N] [--logprobs] [--PARAM VALUE]...
     cima run --random-shape NAME [--weights-seed S] [TOKEN_ID ...] ...
     cima bench <MODEL_DIR> [-n TOKENS] [--iters N] [--batch B] [--prompt-len P]
     cima profile <MODEL_DIR> | --random-shape NAME [--batch B] [--prompt-len P]
@@ -35,6 +35,8 @@ Usage:
        --stream                           print every token as its step is read ("<prompt>:<token>" a line)
        --dtype bfloat16|float32           precision of the whole model (default bfloat16)
        --max-seq N                        positions the cache holds in all (default 8192)
+       --continuations N                  N answers to each prompt, one a line, drawn with seeds that follow --seed (the prompt runs once)
+       --logprobs                         behind each answer, after a tab, the log-probability of its tokens together
        --PARAM VALUE                      generation parameters (see `cima run --help`)
   cima bench <MODEL_DIR> [-n TOKENS] [--iters N] [--batch B] [--prompt-len P]
                                         Greedy decode rate, stop tokens ignored, one discarded warm-up
@@ -72,7 +74,7 @@ def _flag(args: List[str], name: str, default=None):
 
 def cmd_run(args: List[str]) -> int:
     if "--help" in args or "-h" in args:
-        print("usage: cima run <MODEL_DIR> [TOKEN_ID ...] [--prompts FILE] [--dtype D] [--max-seq N] [--PARAM VALUE]...\n")
+        print("usage: cima run <MODEL_DIR> [TOKEN_ID ...] [--prompts FILE] [--dtype D] [--max-seq N] [--continuations N] [--logprobs] [--PARAM VALUE]...\n")
         print(render_help(), end="")
         return 0
     rest = list(args)
@@ -90,6 +92,12 @@ def cmd_run(args: List[str]) -> int:
     dtype = _flag(rest, "--dtype", "bfloat16")
     max_seq = int(_flag(rest, "--max-seq", "8192"))
     prompts_file = _flag(rest, "--prompts")
+    copies = int(_flag(rest, "--continuations", "1"))
+    if copies < 1:
+        raise SystemExit(f"cima run: --continuations {copies}: at least one")
+    scored = "--logprobs" in rest
+    if scored:
+        rest.remove("--logprobs")
     stream = "--stream" in rest
     if stream:
         rest.remove("--stream")
@@ -123,11 +131,11 @@ def cmd_run(args: List[str]) -> int:
         lm = cima_b200.load(config=SHAPES[shape], seed=weights_seed, dtype=dtype, max_tokens=max_seq)
     t0 = time.perf_counter()
     on_token = (lambda i, t: print(f"{i}:{t}", flush=True)) if stream else None
-    results = lm.generate(prompts, opts, on_token=on_token)
+    results = lm.generate(prompts, opts, on_token=on_token, continuations=copies, logprobs=scored)
     total = time.perf_counter() - t0
     if not stream:
         for r in results:
-            print(" ".join(str(t) for t in r.tokens))
+            print(" ".join(str(t) for t in r.tokens) + (f"\t{r.logprob:.6f}" if scored else ""))
     s = lm.stats
     rate = s.gen_tokens / total if total > 0 else 0.0
     print(f"[{s.prompt_tokens} prompt tok | {s.gen_tokens} gen tok | ttft {s.prefill_s * 1e3:.0f} ms | {rate:.1f} tok/s]",

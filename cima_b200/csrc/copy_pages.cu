@@ -8,7 +8,7 @@
 // wait for one, and it can be checked before anything runs (ids inside the storage, no page written twice, none both read and
 // written: the copies of a plan have no order among them).
 //
-// Bound: bytes.  A thread moves four vectors of 16 bytes (less where a position's bytes or the storage are not so aligned), all
+// Bound: bytes.  A thread moves four vectors of 16 bytes (narrower ones where a position's bytes or the storage are not so aligned), all
 // four on their way before the first is written.
 #include "common.cuh"
 #include <stdlib.h>
@@ -87,7 +87,6 @@ extern "C" int cima_copy_pages(void* storage, int layers, long long pages, int s
     return cima_fail(CIMA_E_SIZE, "copy_pages: storage of %d layers, %lld pages, %d segments of %d positions of %lld bytes", layers, pages, segments, page_size, row_bytes);
   if (row_bytes * page_size * segments >= (1ll << 31)) return cima_fail(CIMA_E_SIZE, "copy_pages: a page of %lld bytes; below 2^31 are possible", row_bytes * page_size * segments);
   const int width = (int)((unsigned long long)row_bytes | (unsigned long long)(uintptr_t)storage) & 15;
-  if (width & 1) return cima_fail(CIMA_E_ARG, "copy_pages: the storage and its positions (%lld bytes) must be aligned to 2 bytes", row_bytes);
   const CopyPage* pg = reinterpret_cast<const CopyPage*>(plan);
   unsigned char* seen = (unsigned char*)calloc((size_t)pages, 1);       // 1: read, 2: written
   if (!seen) return cima_fail(CIMA_E_ARG, "copy_pages: no host memory to check a plan over %lld pages", pages);
@@ -106,5 +105,6 @@ extern "C" int cima_copy_pages(void* storage, int layers, long long pages, int s
   if (width == 0) return launch<uint4>(storage, layers, pages, segments, page_size, row_bytes, pg, n, stream);
   if (width == 8) return launch<uint2>(storage, layers, pages, segments, page_size, row_bytes, pg, n, stream);
   if ((width & 3) == 0) return launch<unsigned>(storage, layers, pages, segments, page_size, row_bytes, pg, n, stream);
-  return launch<unsigned short>(storage, layers, pages, segments, page_size, row_bytes, pg, n, stream);
+  if ((width & 1) == 0) return launch<unsigned short>(storage, layers, pages, segments, page_size, row_bytes, pg, n, stream);
+  return launch<unsigned char>(storage, layers, pages, segments, page_size, row_bytes, pg, n, stream);
 }

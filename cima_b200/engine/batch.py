@@ -51,6 +51,7 @@ class StepBatch:
     q_tile_tc_seq: torch.Tensor = None
     q_tile_tc_row0: torch.Tensor = None
     even: bool = True                 # the sequences are of about one length (``lengths_are_even``)
+    shared: Any = None                # ``SharedPrefixes`` of a one-token step whose sequences have pages in common
     host_seq_slot: np.ndarray = None
     host_seq_first_row: np.ndarray = None
     host_seq_len: np.ndarray = None

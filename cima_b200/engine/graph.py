@@ -14,6 +14,7 @@ from typing import List, Sequence
 import numpy as np
 import torch
 
+from ..cache import SharedPrefixes
 from .batch import StepBatch, StepEntry, build_batch
 
 
@@ -32,6 +33,25 @@ def one_token_batch(meta: torch.Tensor, n_seqs: int, max_len: int, even: bool = 
                      seq_len=m[5 * B + 1:6 * B + 1], want_rows=m[2 * B:3 * B], max_rows=1, host_seq_first_row=np.arange(B + 1, dtype=np.int32))
 
 
+def shared_shape(groups) -> tuple:
+    """What a recorded step of sequences that share prefixes fixes of them: (groups, sequences of the largest); () where nothing is shared."""
+    return (len(groups), max(len(members) for members, _ in groups)) if groups else ()
+
+
+class SharedBuffer:
+    """The ``SharedPrefixes`` of a recorded step: arrays of fixed address, filled anew for other sequences of the same ``shared_shape``."""
+
+    def __init__(self, shape: tuple, n_seqs: int, device):
+        n = 2 * n_seqs + 3 * shape[0]
+        self.n_seqs = n_seqs
+        self.device = torch.zeros(n, dtype=torch.int32, device=device)
+        self.shared = SharedPrefixes.over(self.device, n_seqs, shape[1])
+
+    def load(self, groups) -> None:
+        host = torch.from_numpy(SharedPrefixes.pack(groups, self.n_seqs))
+        self.device.copy_(host.pin_memory() if self.device.is_cuda else host, non_blocking=True)
+
+
 def fill_meta(h: np.ndarray, slots: Sequence[int], tokens: Sequence[int], lengths: Sequence[int]) -> None:
     """Sequence i sits in slots[i], holds lengths[i] positions and brings tokens[i]."""
     B = len(slots)
@@ -47,11 +67,12 @@ class DecodeGraph:
     """One batch size's captured step.  ``load`` sets its inputs for a set of sequences; ``run``
     does one step (the first run after construction executes eagerly and captures)."""
 
-    def __init__(self, model, sampler, n_seqs: int, all_greedy: bool, max_len: int = 0, pool=None):
+    def __init__(self, model, sampler, n_seqs: int, all_greedy: bool, max_len: int = 0, pool=None, shape: tuple = (), logprobs: bool = False):
         """``max_len``: the most positions that a sequence may hold after a step of this graph (0: as many as the model
         takes; ``UNEVEN``: the same, of sequences far from one length).  A recorded step fixes its launches; one recorded for short
         or middling contexts takes the kernels' choices for them, and the stepper moves on to the next graph when a sequence outgrows the bound.  ``pool``: the memory that its
-        recording shares with others (of the same caller: they run one after another, and nothing in it outlives a step)."""
+        recording shares with others (of the same caller: they run one after another, and nothing in it outlives a step).  ``shape``: the
+        ``shared_shape`` of sequences that share prefixes.  ``logprobs``: the chosen tokens' log-probabilities stand behind the tokens in ``result``."""
         self.model, self.sampler = model, sampler
         self.B = B = n_seqs
         self.all_greedy = all_greedy
@@ -64,12 +85,19 @@ class DecodeGraph:
         self.tokens, self.row_pos, self.row_seq = b.tokens, b.row_pos, b.row_seq
         self.seq_slot, self.seq_first_row, self.seq_len = b.seq_slot, b.seq_first_row, b.seq_len
         self.params = torch.zeros(B, 4, dtype=torch.float32, device=dev)
-        self.chosen = torch.zeros(B, dtype=torch.int32, device=dev)
+        self.shared = SharedBuffer(shape, B, dev) if shape else None
+        if self.shared is not None:
+            b.shared = self.shared.shared
+        self.result = torch.zeros(2 * B if logprobs else B, dtype=torch.int32, device=dev)
+        self.chosen = self.result[:B]
+        self.logprobs = self.result[B:].view(torch.float32) if logprobs else None
         self.graph = None
         self.slots: List[int] = []
 
-    def load(self, slots: Sequence[int], tokens: Sequence[int], lengths: Sequence[int], params: np.ndarray) -> None:
-        """Inputs of the next step: sequence i sits in slots[i], holds lengths[i] positions and brings tokens[i]."""
+    def load(self, slots: Sequence[int], tokens: Sequence[int], lengths: Sequence[int], params: np.ndarray, groups=()) -> None:
+        """Inputs of the next step: sequence i sits in slots[i], holds lengths[i] positions and brings tokens[i]; ``groups``: what they share."""
+        if self.shared is not None:
+            self.shared.load(groups)
         fill_meta(self.meta_host.numpy(), slots, tokens, lengths)
         self.meta.copy_(self.meta_host, non_blocking=True)
         self.params.copy_(torch.from_numpy(params), non_blocking=False)
@@ -86,6 +114,8 @@ class DecodeGraph:
     def _step(self) -> None:
         logits = self.model.forward(self.batch)
         self.sampler.sample(logits, self.seq_slot, self.params, self.chosen, self.all_greedy)
+        if self.logprobs is not None:
+            self.model.rt.kernels.token_logprobs(logits, self.chosen, self.logprobs)
         self.model.rt.kernels.decode_advance(self.chosen, self.tokens, self.row_pos, self.seq_len)
 
     def run(self) -> torch.Tensor:
@@ -196,22 +226,27 @@ class StepGraph:
     its memory is given back with the last reference to it.)  A model's recordings share one pool of memory, and one stream to be
     recorded on: they run one after another, and nothing but their logits outlives a replay (``engine.fit`` counts both)."""
 
-    def __init__(self, model, n_seqs: int, max_len: int):
+    def __init__(self, model, n_seqs: int, max_len: int, shape: tuple = ()):
         self.n_seqs = n_seqs
         self.meta = torch.zeros(6 * n_seqs + 1, dtype=torch.int32, device=model.rt.device)
         self.batch = one_token_batch(self.meta, n_seqs, max_len if max_len > 0 else model.most_positions, max_len != UNEVEN)
+        self.shared = SharedBuffer(shape, n_seqs, model.rt.device) if shape else None
+        if self.shared is not None:
+            self.batch.shared = self.shared.shared
         self.graph = None
         self.logits = None
         self.uses = 0
         self.last = 0                              # number of the model's one-token step that used it last
         self.recordable = True
 
-    def run(self, model, slots: Sequence[int], tokens: Sequence[int], lengths: Sequence[int]) -> torch.Tensor:
+    def run(self, model, slots: Sequence[int], tokens: Sequence[int], lengths: Sequence[int], groups=()) -> torch.Tensor:
         """Float32 logits [sequences, vocab].  The caller has reserved the new position of every slot and commits it, then asks for
         the recording (``record``)."""
         host = torch.empty(6 * self.n_seqs + 1, dtype=torch.int32, pin_memory=True)      # its own each time: the copy may still be under way
         fill_meta(host.numpy(), slots, tokens, lengths)
         self.meta.copy_(host, non_blocking=True)
+        if self.shared is not None:
+            self.shared.load(groups)
         if self.graph is not None:
             self.graph.replay()
             return self.logits.clone()

@@ -17,7 +17,7 @@ from typing import Dict, List, Optional, Sequence
 
 import torch
 
-from ..cache.kv import KVCache, StateRequest
+from ..cache.kv import KVCache, SharedPrefixes, StateRequest
 from ..config.registry import lookup_architecture, read_config_json
 from ..config.specs import ModelSpec
 from ..parts import Linear, Runtime, build_block, build_norm
@@ -25,7 +25,7 @@ from ..parts.linear import FOLDED_NORM_ROWS
 from ..parts.norm import RowsInfo
 from ..weights.loader import TensorSpec, tensor_names
 from .batch import StepBatch, StepEntry, build_batch, check_entries, lengths_are_even
-from .graph import UNEVEN
+from .graph import UNEVEN, shared_shape
 from .fit import STEP_ROWS
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32,
@@ -36,6 +36,11 @@ def parse_dtype(d) -> torch.dtype:
     if d not in _DTYPES:
         raise ValueError(f"dtype {d!r} is not one of bfloat16, float32")
     return _DTYPES[d]
+
+
+def worth_sharing(groups, page_size: int) -> bool:
+    """Whether a step's attention is the shorter for reading the groups' prefixes once."""
+    return bool(groups)
 
 
 def build_plan(spec: ModelSpec, rt: Optional[Runtime] = None) -> Dict[str, TensorSpec]:
@@ -228,7 +233,7 @@ class Model:
         self.cache = KVCache(self._cache_requests(),
                              max_tokens, self.spec.max_position,
                              self.rt.dtype, self.rt.device, page_size=page_size, max_seqs=max_seqs,
-                             shares=shares, extra_state=extra_state)
+                             shares=shares, extra_state=extra_state, kernels=self.rt.kernels)
         return self.cache
 
     BIGRAM_STATE = "embed.bigram_prev"
@@ -282,12 +287,16 @@ class Model:
         limit = cache.most_tokens_going_on()
         if limit is not None and any(starts) and max(len(e.tokens) for e in entries) > limit:
             return self._step_in_rounds(entries, limit)
+        groups = self.shared_groups([e.slot for e in entries]) if all(len(e.tokens) == 1 for e in entries) else []
         if record and self._recordable(entries):
             with self._step_lock:
-                g = self._step_graph([n + 1 for n in starts])
+                g = self._step_graph([n + 1 for n in starts], shared_shape(groups))
                 if g is not None:
-                    return self._step_recorded(g, entries, starts)
+                    return self._step_recorded(g, entries, starts, groups)
         batch = build_batch(entries, starts, self.spec.vocab, self.rt.device)
+        if groups:
+            packed = torch.from_numpy(SharedPrefixes.pack(groups, len(entries))).to(self.rt.device)
+            batch.shared = SharedPrefixes.over(packed, len(entries), shared_shape(groups)[1])
         for e, s in zip(entries, starts):
             cache.reserve(e.slot, s + len(e.tokens))
         cache.flush()
@@ -295,6 +304,11 @@ class Model:
         for e, s in zip(entries, starts):
             cache.commit(e.slot, s + len(e.tokens))
         return logits
+
+    def shared_groups(self, slots: Sequence[int]):
+        """What a one-token step of ``slots`` may read once for several of them (``KVCache.shared_groups``), where that is worth it."""
+        groups = self.cache.shared_groups(slots)
+        return groups if worth_sharing(groups, self.cache.page_size) else []
 
     def _recordable(self, entries: Sequence[StepEntry]) -> bool:
         """Whether the step runs through a ``StepGraph``: one token a sequence, every sequence's logits wanted, parts that may
@@ -304,13 +318,14 @@ class Model:
                 and self.graph_safe and torch.device(self.rt.device).type == "cuda" and getattr(self.rt.kernels, "profile", None) is None
                 and not torch.cuda.is_current_stream_capturing())
 
-    def _step_graph(self, lengths: Sequence[int]):
+    def _step_graph(self, lengths: Sequence[int], shape: tuple = ()):
         """The ``StepGraph`` of a step that leaves ``lengths``, or None where as many others as are kept have been in use of late: a caller
         that goes round among more shapes replays some and issues the rest, rather than recording each anew.  A batch size takes no more than its
         share then: one recorded for longer contexts serves the shorter ones too, and takes their recording's place."""
         from . import graph
         graphs = self._step_graphs
-        key = (len(lengths), self.context_bound(lengths))
+        # (sequences that share prefixes have recordings of their own: (sequences, groups, most of a group) stands where the sequences do)
+        key = ((len(lengths), *shape) if shape else len(lengths), self.context_bound(lengths))
         self._steps += 1
         g = graphs.get(key)
         if g is None:
@@ -329,7 +344,7 @@ class Model:
                 torch.cuda.synchronize()
                 graphs.popitem(last=False)
         if g is None:
-            g = graphs[key] = graph.StepGraph(self, *key)
+            g = graphs[key] = graph.StepGraph(self, len(lengths), key[1], shape) if shape else graph.StepGraph(self, *key)
         graphs.move_to_end(key)
         g.last = self._steps
         return g
@@ -346,7 +361,7 @@ class Model:
             self._step_pool = (torch.cuda.graph_pool_handle(), torch.cuda.Stream())
         return self._step_pool
 
-    def _step_recorded(self, g, entries: Sequence[StepEntry], starts: Sequence[int]) -> torch.Tensor:
+    def _step_recorded(self, g, entries: Sequence[StepEntry], starts: Sequence[int], groups=()) -> torch.Tensor:
         check_entries(entries, self.spec.vocab)
         cache = self.cache
         # The recordings' inputs and memory serve every stream and thread: a step waits for the one before it, wherever that ran.
@@ -359,7 +374,7 @@ class Model:
             cache.reserve(e.slot, s + 1)
         cache.flush()
         try:
-            logits = g.run(self, [e.slot for e in entries], [int(e.tokens[0]) for e in entries], starts)
+            logits = g.run(self, [e.slot for e in entries], [int(e.tokens[0]) for e in entries], starts, groups)
         finally:
             self._step_done.record(stream)
         for e, s in zip(entries, starts):

@@ -13,7 +13,7 @@ from ..cache.kv import CapacityError
 from ..sampling.options import GenOptions
 from ..sampling.sampler import DeviceSampler
 from .batch import StepEntry
-from .graph import MAX_PROMPT_GRAPHS
+from .graph import MAX_PROMPT_GRAPHS, shared_shape
 
 
 MIN_REUSE = 16     # a finished sequence is taken up again only for at least this many tokens in common
@@ -47,7 +47,11 @@ class ModelStepper:
         from .graph import recorded_prompt_rows
         self.prompt_rows = (recorded_prompt_rows(model.weight_bytes(), len(model.spec.schedule), (4 if model.rt.dtype is torch.float32 else 2))
                             if self.use_graphs else 0)
-        self._armed = None            # (graph, slots) whose device-side inputs are those of the next step
+        self.logprobs = False         # whether ``last_logprobs`` is wanted (the loop says so before a batch)
+        self.last_logprobs: List[float] = []     # log-probabilities of the tokens that ``prefill`` or ``decode`` returned last, before penalty,
+                                      # temperature and cuts
+        self._adopted = {}            # slot -> positions that it goes back to (``adopt``), until it runs
+        self._armed = None            # (graph's key, slots, what they share) whose device-side inputs are those of the next step
         cache = model.cache
         self.max_batch = max(1, min(max_batch, cache.n_slots))
         self.sampler = DeviceSampler(model, max_rows=self.max_batch)
@@ -90,6 +94,7 @@ class ModelStepper:
                     best, best_n = slot, n
             if best is not None:
                 del self._retained[best]
+                self._adopted[best] = best_n
             out.append((best, best_n))
         return out
 
@@ -101,7 +106,7 @@ class ModelStepper:
         want = 0
         for need, slot in zip(needs, slots):
             pages = -(-need // page) * page
-            want += pages if slot is None else max(0, pages - cache.held_tokens(slot))
+            want += pages if slot is None else max(0, pages - cache.held_tokens(slot)) + cache.shared_tokens(slot, self._adopted.get(slot, 0), need)
         while self._retained and cache.free_tokens() < want:
             self._evict_oldest()
 
@@ -121,35 +126,85 @@ class ModelStepper:
         while self._retained:
             self._evict_oldest()
 
+    def fork(self, slot: int, count: int) -> List[int]:
+        """``count`` slots that go on from where ``slot`` is (``KVCache.fork``)."""
+        cache = self.model.cache
+        while cache.slots.free < count and self._retained:
+            self._evict_oldest()
+        return cache.fork(slot, count)
+
+    def shared_positions(self, length: int) -> int:
+        """Positions of a prompt of ``length`` tokens that its further continuations need no pages for (none where a group keeps a ring)."""
+        cache = self.model.cache
+        return 0 if any(g.ring_pages for g in cache.groups) else length // cache.page_size * cache.page_size
+
     def prefill(self, slots, prompts, options, reused: Optional[Sequence[int]] = None) -> List[int]:
         """The prompts' step.  ``reused[i]`` > 0: slot i already holds that many of prompt i's tokens (``adopt``)."""
+        reused = self._begin_prompts(slots, reused)
+        self.sampler.begin(slots, prompts, options)
+        if not any(reused):
+            logits = self._short_prompts(slots, prompts)
+            if logits is not None:
+                return self._choose(logits, slots, options, sum(len(p) for p in prompts))
+        out: List[Optional[int]] = [None] * len(slots)
+        lps: List[float] = [0.0] * len(slots)
+        for group, logits in self._prompt_steps(slots, prompts, reused):
+            toks = self._choose(logits, [slots[i] for i in group], [options[i] for i in group], sum(len(prompts[i]) - reused[i] for i in group))
+            for i, t in zip(group, toks):
+                out[i] = t
+            for i, p in zip(group, self.last_logprobs):
+                lps[i] = p
+        self.last_logprobs = lps if self.logprobs else []
+        return out  # type: ignore[return-value]
+
+    def prefill_copies(self, slots, prompts, options, copies: Sequence[int], reused: Optional[Sequence[int]] = None):
+        """``prefill`` where ``copies[i]`` >= 1 sequences go on from prompt i: each prompt runs once, in slots[i], and is forked for its
+        others; ``options`` holds an entry for each sequence, prompt by prompt.  Returns (slots, first tokens) of all of them in that order, the
+        tokens of a prompt's sequences chosen from the same logits.  The further slots are the caller's to close; none is left open if this raises."""
+        reused = self._begin_prompts(slots, reused)
+        logits = None if any(reused) else self._short_prompts(slots, prompts)
+        if logits is None:
+            steps = list(self._prompt_steps(slots, prompts, reused))
+            row = {i: r for r, i in enumerate(i for group, _ in steps for i in group)}
+            logits = torch.cat([lg for _, lg in steps])
+        else:
+            row = {i: i for i in range(len(slots))}
+        every: List[int] = []
+        forked: List[int] = []
+        try:
+            for s, n in zip(slots, copies):
+                self.model.cache.trim(s)              # a recorded prompt step's padding is room that the others may need
+                more = self.fork(s, n - 1)
+                forked += more
+                every += [s] + more
+            self.sampler.begin(every, [p for p, n in zip(prompts, copies) for _ in range(n)], options)
+            rows = torch.as_tensor([row[i] for i, n in enumerate(copies) for _ in range(n)], dtype=torch.int32, device=logits.device)
+            each = torch.empty((len(every), logits.shape[1]), dtype=torch.float32, device=logits.device)
+            self.model.rt.kernels.gather_rows(logits, rows, each)
+            return every, self._choose(each, every, options, sum(len(p) - n for p, n in zip(prompts, reused)))
+        except BaseException:
+            self.model.cache.close(forked)
+            raise
+
+    def _begin_prompts(self, slots, reused: Optional[Sequence[int]]) -> List[int]:
         self._drain()
         self._armed = None
-        self.sampler.begin(slots, prompts, options)
         reused = list(reused) if reused is not None else [0] * len(slots)
-        cache = self.model.cache
         for s, n in zip(slots, reused):
+            self._adopted.pop(s, None)
             if n:
-                cache.rewind(s, n)
-        if not any(reused):
-            first = self._short_prompts(slots, prompts, options)
-            if first is not None:
-                return first
-        out: List[Optional[int]] = [None] * len(slots)
+                self.model.cache.rewind(s, n)
+        return reused
+
+    def _prompt_steps(self, slots, prompts, reused):
         # sequences that start run as one prompt step (attention over the step's own keys), those that go on as
         # another (rows that read the cache)
         for group in ([i for i, n in enumerate(reused) if not n], [i for i, n in enumerate(reused) if n]):
-            if not group:
-                continue
-            entries = [StepEntry(slots[i], prompts[i][reused[i]:], [len(prompts[i]) - reused[i] - 1]) for i in group]
-            toks = self._choose(self.model.step(entries), [slots[i] for i in group], [options[i] for i in group],
-                                sum(len(e.tokens) for e in entries))
-            for i, t in zip(group, toks):
-                out[i] = t
-        return out  # type: ignore[return-value]
+            if group:
+                yield group, self.model.step([StepEntry(slots[i], prompts[i][reused[i]:], [len(prompts[i]) - reused[i] - 1]) for i in group])
 
-    def _short_prompts(self, slots, prompts, options) -> Optional[List[int]]:
-        """The first tokens of a few short prompts through a recorded step (``PromptGraph``), or None where that
+    def _short_prompts(self, slots, prompts) -> Optional[torch.Tensor]:
+        """The logits behind a few short prompts through a recorded step (``PromptGraph``), or None where that
         does not apply: graphs off, prompts beyond the largest bucket or more rows than a recorded step takes, no
         room for the bucket's rows, a mixer that keeps state of its own per sequence (the padding's rows would pass
         through it), or a group of layers that keeps a window's keys in a ring of pages (the padding's keys would
@@ -184,7 +239,7 @@ class ModelStepper:
         logits = g.run(slots, prompts)
         for s, p in zip(slots, prompts):
             cache.commit(s, len(p))
-        return self._choose(logits, slots, options, sum(len(p) for p in prompts))
+        return logits
 
     def decode(self, slots, last_tokens, options) -> List[int]:
         if not self.use_graphs:
@@ -193,13 +248,13 @@ class ModelStepper:
         if not self.pipeline:
             graph = self._arm(slots, last_tokens, options)
             self.reserve_ahead(slots, 1)
-            chosen = graph.run()
-            view = self._pinned_view(len(slots))
-            view.copy_(chosen, non_blocking=True)    # the step's result crosses to the host here, into pinned memory
+            graph.run()
+            view = self._pinned_view(graph.result.numel())
+            view.copy_(graph.result, non_blocking=True)    # the step's result crosses to the host here, into pinned memory
             torch.cuda.current_stream().synchronize()
-            out = view.tolist()
+            out, self.last_logprobs = self._split(view, len(slots))
             self._advance_lengths(slots, 1)
-            self.d2h_bytes += 4 * len(slots)
+            self.d2h_bytes += 4 * view.numel()
             return out
         return self._decode_pipelined(tuple(slots), list(last_tokens), options)
 
@@ -221,14 +276,14 @@ class ModelStepper:
         except (CacheFull, CapacityError):
             return None
         cache.flush()
-        chosen = graph.run()
-        view = self._pinned_view(len(slots))
-        view.copy_(chosen, non_blocking=True)
+        graph.run()
+        view = self._pinned_view(graph.result.numel())
+        view.copy_(graph.result, non_blocking=True)
         ev = torch.cuda.Event()
         ev.record()
         for s in slots:
             self._inflight[s] = self._inflight.get(s, 0) + 1
-        self.d2h_bytes += 4 * len(slots)
+        self.d2h_bytes += 4 * view.numel()
         return {"slots": slots, "graph": graph, "tokens": view, "event": ev, "fed": None}
 
     def _pinned_view(self, n: int) -> torch.Tensor:
@@ -239,9 +294,16 @@ class ModelStepper:
             self._pinned[i] = torch.empty(max(64, n), dtype=torch.int32).pin_memory()
         return self._pinned[i][:n]
 
+    @staticmethod
+    def _split(view: torch.Tensor, n: int):
+        """(tokens, their log-probabilities or none) of a step's result on the host."""
+        return view[:n].tolist(), view[n:].view(torch.float32).tolist()
+
     def _read(self, flight, commit_slots) -> List[int]:
         flight["event"].synchronize()
-        toks = flight["tokens"].tolist()
+        toks, lps = self._split(flight["tokens"], len(flight["slots"]))
+        at = {s: i for i, s in enumerate(flight["slots"])}
+        self.last_logprobs = [lps[at[s]] for s in commit_slots] if lps else []
         cache = self.model.cache
         for s in flight["slots"]:
             self._inflight[s] -= 1
@@ -265,7 +327,7 @@ class ModelStepper:
 
     def _decode_pipelined(self, slots, last_tokens, options) -> List[int]:
         fl = self._flight
-        if fl is not None and fl["fed"] is not None and set(slots) <= set(fl["slots"]) and \
+        if fl is not None and fl["fed"] is not None and (fl["graph"].logprobs is not None) == self.logprobs and set(slots) <= set(fl["slots"]) and \
                 all(fl["fed"][s] == t for s, t in zip(slots, last_tokens)):
             if fl["slots"] == slots and self._context_bound(slots, 1) == fl["graph"].max_len:
                 nxt = self._launch(fl["graph"], slots)           # the step after, before this one is read
@@ -305,12 +367,14 @@ class ModelStepper:
         cache = self.model.cache
         all_greedy = all(o.greedy for o in options)
         bound = self._context_bound(slots, ahead)
-        key = (len(slots), all_greedy, bound)
+        armed = self._armed[1:] if self._armed and self._armed[1] == tuple(slots) else None
+        groups = armed[1] if armed else self.model.shared_groups(slots)      # (what is shared stays shared while these sequences go on)
+        key = (len(slots), all_greedy, bound, shared_shape(groups), self.logprobs)
         graph = self._graphs.get(key)
         if graph is None:
             from .graph import DecodeGraph
-            graph = self._graphs[key] = DecodeGraph(self.model, self.sampler, len(slots), all_greedy, bound, self._graph_pool)
-        if self._armed != (key, tuple(slots)):
+            graph = self._graphs[key] = DecodeGraph(self.model, self.sampler, len(slots), all_greedy, bound, self._graph_pool, key[3], self.logprobs)
+        if self._armed is None or self._armed[:2] != (key, tuple(slots)):
             params = np.array([[o.temperature, float(o.top_k), o.top_p, o.repeat_penalty] for o in options], dtype=np.float32)
             carried = None
             if last_tokens is None:
@@ -319,11 +383,11 @@ class ModelStepper:
                 if before is None:
                     raise ValueError("the next step's tokens are needed: no recorded step of these sequences holds them")
                 carried = before.tokens.clone()
-            graph.load(slots, last_tokens if carried is None else [0] * len(slots), [cache.length(s) for s in slots], params)
+            graph.load(slots, last_tokens if carried is None else [0] * len(slots), [cache.length(s) for s in slots], params, groups)
             if carried is not None:
                 graph.tokens.copy_(carried)
             self.h2d_bytes += 4 * (6 * len(slots) + 1) + params.nbytes
-            self._armed = (key, tuple(slots))
+            self._armed = (key, tuple(slots), groups)
         elif last_tokens is not None:
             graph.feed(last_tokens)
             self.h2d_bytes += 4 * len(slots)
@@ -373,6 +437,12 @@ class ModelStepper:
             self.sampler.sample(logits, row_slot, DeviceSampler.params(options, dev), tokens, False)
         self.h2d_bytes += 4 * (3 * tokens_in + 3 * n + 1 + n)
         self.d2h_bytes += 4 * n
+        lps = None
+        if self.logprobs:
+            lps = torch.empty(n, dtype=torch.float32, device=dev)
+            self.model.rt.kernels.token_logprobs(logits, tokens, lps)
+            self.d2h_bytes += 4 * n
         out = tokens.tolist()
+        self.last_logprobs = lps.tolist() if lps is not None else []
         self.model.check_device()
         return out

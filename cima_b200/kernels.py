@@ -670,6 +670,12 @@ class Kernels:
         also holds exp(head_sink[h]), an entry that is not scaled and carries no value.  ``gate_col`` > 0: a row of ``qkv`` holds
         one gate value for each value of its result from that column on, and the result leaves times their sigmoid.  ``slopes`` (float32 [n_heads]): slopes[h] * (i - j) is taken
         off the scaled score of the query at position i with the key at j."""
+        shared = getattr(batch, "shared", None)
+        if (shared is not None and from_cache and batch.n_rows == batch.n_seqs and window <= 0 and v_group == 1 and kv.page_size == 64
+                and kv.ring_pages == 0 and head_dim % (16 if qkv.dtype is torch.bfloat16 else 4) == 0 and head_dim <= 128):
+            return self.attention_shared(qkv, kv, batch.seq_slot, batch.seq_len, shared, out, n_heads, n_kv_heads, head_dim, scale,
+                                         int(getattr(batch, "max_len", 0) or 0), early=after_append, sink=sink, head_sink=head_sink, gate_col=gate_col,
+                                         slopes=slopes)
         if (from_cache and qkv.dtype is torch.bfloat16 and kv.page_size == 64 and head_dim % 16 == 0
                 and head_dim <= 128 and batch.n_rows == batch.n_seqs):
             plain = not (sink or keep_first or v_group > 1 or head_sink is not None or gate_col or slopes is not None)
@@ -904,7 +910,7 @@ class Kernels:
     # ------------------------------------------------------------------ pages
     def copy_pages(self, storage: torch.Tensor, plan: torch.Tensor) -> None:
         """storage[:, to, :, :, :n] = storage[:, from, :, :, :n] for each (from, to, n) of ``plan`` (int32 [entries, 3] on the host), in one launch
-        for up to 320 entries.  ``storage`` [layers, pages, planes, heads, positions, values], any element type of 2 bytes or more (bits are
+        for up to 320 entries.  ``storage`` [layers, pages, planes, heads, positions, values], any element type (bits are
         moved).  No page may be written twice, or both read and written: the copies have no order among them."""
         self._need(storage, "storage", None, 6)
         self._here(storage)
