@@ -117,15 +117,22 @@ def extend_splits(blocks: int, max_len: int, window: int, keep_first: int) -> in
     return max(1, min(64, tiles // 4, EXTEND_BLOCKS // max(1, blocks)))
 
 
-def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_heads: int, max_len: int) -> Tuple[int, int]:
-    """(splits of a group's prefix, splits of a sequence's own pages) of ``Kernels.attention_shared``: about one wave of blocks for each."""
-    group = n_heads // n_kv_heads
-    rows = most * group
-    tile = 16 if rows <= 16 else 32 if rows <= 32 else 64
-    pages = -(-max_len // 64) if max_len > 0 else 1 << 20
-    prefix = n_groups * -(-rows // tile) * n_kv_heads
-    own = n_seqs * n_kv_heads * -(-group // 16)
-    return (max(1, min(64, SPLIT_BLOCKS // max(1, prefix), pages)), max(1, min(32, SPLIT_BLOCKS // own, pages)))
+SHARED_TC_ROWS = 16         # query rows a kv head of the largest group, above which prefixes run on tcgen05 (blocks of 128 rows)
+
+
+def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_heads: int, max_len: int, rows: int = 128) -> Tuple[int, int]:
+    """(splits of a group's prefix, splits of a sequence's own pages) of ``Kernels.attention_shared``; the kernel leaves those without work that would have
+    less than two pages (on tcgen05; else one), but a block without work still has to be placed.  ``rows``: query rows of a block of a prefix.  Prefixes: one wave of blocks (two
+    an SM).  Own pages, of which there mostly are few: some 64 blocks, at least one a sequence and kv head; where sequences share nothing (there are more
+    than the groups can hold) theirs are as long as the longest, and a block should have about 8 of them, in four waves at most."""
+    group, pages = n_heads // n_kv_heads, (max_len + 63) // 64 if max_len > 0 else 1 << 16
+    prefix = n_groups * -(-most * group // rows) * n_kv_heads
+    blocks = n_seqs * n_kv_heads * -(-group // 16)
+    own = min(4, 64 // blocks)
+    if n_seqs > n_groups * most:
+        own = max(own, min(16, pages // 8, 4 * SPLIT_BLOCKS // blocks))
+    least = 2 if rows == 128 else 1
+    return max(1, min(48, SPLIT_BLOCKS // max(1, prefix), pages // least)), max(1, min(own, pages // least))
 
 
 # epilogues of the skinny product
@@ -175,6 +182,8 @@ _SIGNATURES = {
     "cima_attention_decode_near_room": [_i, _vp],
     "cima_attention_shared": [_vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _f, _f, _vp, _i,
                               _vp, _i, _vp],
+    "cima_attention_shared_tc": [_vp, _i, _vp, ctypes.c_longlong, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i,
+                                 _i, _f, _f, _vp, _i, _vp, _i, _vp, _vp],
     "cima_attention_prefill": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _f, _i, _i, _vp, _i, _vp, _vp],
     "cima_attention_extend": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _f, _i, _i, _vp, _i, _vp,
                               _i, _vp, _vp, _vp],
@@ -872,39 +881,56 @@ class Kernels:
 
     def attention_shared(self, qkv: torch.Tensor, kv, seq_slot, seq_len, shared, out: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
                          scale: float, max_len: int = 0, early: bool = False, sink: float = 0.0, head_sink=None, gate_col: int = 0, slopes=None,
-                         splits: Optional[Tuple[int, int]] = None) -> None:
+                         splits: Optional[Tuple[int, int]] = None, tc: Optional[bool] = None) -> None:
         """One query per sequence over the paged cache where groups of sequences hold the same pages for a prefix (``shared``, a
         ``SharedPrefixes``): a group's prefix is read once for all its sequences.  bfloat16 (head sizes that are multiples of 16) or float32
         (multiples of 4) up to 128, pages of 64, every key visible; ``max_len``: positions of the longest sequence (0: not known; it bounds the
-        splits); the other arguments are ``attention_decode``'s."""
-        self._need(qkv, "qkv", None, 2); self._need(out, "out", qkv.dtype, 2)
-        self._need(kv.storage, "cache", qkv.dtype, 5); self._need(kv.block_table, "block_table", torch.int32, 2)
-        B, groups = qkv.shape[0], shared.groups
-        for n, t in (("seq_slot", seq_slot), ("seq_len", seq_len), ("order", shared.order), ("own_page", shared.own_page)):
-            self._need(t, n, torch.int32, 1)
-            if t.numel() < B:
-                raise KernelError(f"attention_shared: {n} has {t.numel()} entries for {B} sequences")
-        self._need(groups, "groups", torch.int32, 2)
-        self._here(qkv, out, kv.storage, kv.block_table, seq_slot, seq_len, shared.order, shared.own_page, groups)
-        self._need_head_sink(head_sink, n_heads, slopes)
+        splits); ``tc``: the prefixes on tcgen05 (None: where that is possible and there are rows for it); the other arguments are ``attention_decode``'s."""
+        storage, table, order, own_page, groups = kv.storage, kv.block_table, shared.order, shared.own_page, shared.groups
+        (B, ld), dtype, at = qkv.shape, qkv.dtype, torch.cuda.current_device()
+        # (one glance at what is right of nearly every call; what is wrong is then named.  The host's time is most of a small step's.)
+        ints = (table, seq_slot, seq_len, order, own_page, groups)
+        if not (all([t.dtype is torch.int32 and t.is_contiguous() and t.get_device() == at for t in ints])
+                and all([t.dtype is dtype and t.is_contiguous() and t.get_device() == at for t in (qkv, out, storage)])
+                and storage.dim() == 5 and table.dim() == 2 and groups.dim() == 2):
+            self._need(qkv, "qkv", None, 2); self._need(out, "out", dtype, 2); self._need(storage, "cache", dtype, 5)
+            for n, t, d in (("block_table", table, 2), ("seq_slot", seq_slot, 1), ("seq_len", seq_len, 1), ("order", order, 1), ("own_page", own_page, 1), ("groups", groups, 2)):
+                self._need(t, n, torch.int32, d)
+            self._here(qkv, out, storage, *ints)
+        if min(seq_slot.numel(), seq_len.numel(), order.numel(), own_page.numel()) < B:
+            raise KernelError(f"attention_shared: slots, lengths, order or own pages have fewer entries than the {B} sequences")
+        if head_sink is not None or slopes is not None:
+            self._need_head_sink(head_sink, n_heads, slopes)
+            self._here(*[t for t in (head_sink, slopes) if t is not None])
         if kv.ring_pages or kv.window:
             raise KernelError("attention_shared: a layer with a window keeps no prefix to share")
-        if tuple(out.shape) != (B, n_heads * head_dim) or tuple(kv.storage.shape[1:]) != (kv.planes, n_kv_heads, kv.page_size, head_dim):
-            raise KernelError(f"attention_shared: out {tuple(out.shape)} or cache pages {tuple(kv.storage.shape)} do not fit {B} rows of {n_heads} heads of {head_dim}")
-        if groups.shape[1] != 3 or qkv.shape[1] < n_heads * head_dim:
-            raise KernelError(f"attention_shared: groups {tuple(groups.shape)} are not [groups, 3], or rows of {qkv.shape[1]} hold no {n_heads} heads of {head_dim}")
-        n_groups, most = groups.shape[0], shared.most
-        np_, no = splits or shared_splits(n_groups, most, B, n_heads, n_kv_heads, max_len)
-        if not self._admit(f"attention_shared[{np_} + {no} splits]", *self._attention_work(qkv, n_heads, n_kv_heads, head_dim, kv.planes)): return
+        pages, *page = storage.shape
+        if out.shape != (B, n_heads * head_dim) or page != [kv.planes, n_kv_heads, kv.page_size, head_dim]:
+            raise KernelError(f"attention_shared: out {tuple(out.shape)} or cache pages {tuple(storage.shape)} do not fit {B} rows of {n_heads} heads of {head_dim}")
+        n_groups, three = groups.shape
+        if three != 3 or ld < n_heads * head_dim:
+            raise KernelError(f"attention_shared: groups {tuple(groups.shape)} are not [groups, 3], or rows of {ld} hold no {n_heads} heads of {head_dim}")
+        most = shared.most
+        if tc is None:                                    # (the flag of the bounded waits lies on the device that first asked for it)
+            tc = (most * (n_heads // n_kv_heads) > SHARED_TC_ROWS and dtype is torch.bfloat16 and head_dim in (64, 128) and ld % 8 == 0
+                  and qkv.data_ptr() % 16 == 0 and pages * kv.planes * n_kv_heads * kv.page_size < 2 ** 31 and self.error_flag(qkv.device).get_device() == at)
+        elif tc and dtype is not torch.bfloat16:
+            raise KernelError(f"attention_shared: {dtype} on tcgen05; it takes bfloat16")
+        np_, no = splits or shared_splits(n_groups, most, B, n_heads, n_kv_heads, max_len, 128 if tc else 32 if dtype is torch.float32 else 16)
+        if self.profile is not None and not self._admit(f"attention_shared[{np_} + {no} splits]", *self._attention_work(qkv, n_heads, n_kv_heads, head_dim, kv.planes)): return
         # this call's own, as attention_decode's
         cells = B * n_heads * (np_ + no)
-        part = torch.empty(cells * (head_dim + 2), dtype=torch.float32, device=qkv.device)
-        at = part.data_ptr()
-        self._check(self.lib.cima_attention_shared(
-            qkv.data_ptr(), dtype_code(qkv.dtype), qkv.shape[1], kv.storage.data_ptr(), kv.block_table.data_ptr(), kv.block_table.shape[1], kv.page_size,
-            kv.planes, seq_slot.data_ptr(), seq_len.data_ptr(), shared.order.data_ptr(), shared.own_page.data_ptr(), groups.data_ptr(), n_groups, most,
-            at, at + 4 * cells * head_dim, np_, no, out.data_ptr(), out.shape[1], B, n_heads, n_kv_heads, head_dim, scale, sink, _ptr(head_sink),
-            gate_col, _ptr(slopes), int(early), self._stream()), "attention_shared")
+        part = torch.empty(cells * (head_dim + 2), dtype=torch.float32, device=qkv.device).data_ptr()
+        rest = (seq_slot.data_ptr(), seq_len.data_ptr(), order.data_ptr(), own_page.data_ptr(), groups.data_ptr(), n_groups, most, part, part + 4 * cells * head_dim,
+                np_, no, out.data_ptr(), out.shape[1], B, n_heads, n_kv_heads, head_dim, scale, sink, _ptr(head_sink), gate_col, _ptr(slopes), int(early))
+        if tc:
+            flag = self.error_flag(qkv.device)
+            self._here(flag)
+            self._check(self.lib.cima_attention_shared_tc(qkv.data_ptr(), ld, storage.data_ptr(), pages, table.data_ptr(), table.shape[1], kv.page_size, kv.planes,
+                                                          *rest, flag.data_ptr(), _raw_stream(at)), "attention_shared_tc")
+        else:
+            self._check(self.lib.cima_attention_shared(qkv.data_ptr(), F32 if dtype is torch.float32 else dtype_code(dtype), ld, storage.data_ptr(), table.data_ptr(),
+                                                       table.shape[1], kv.page_size, kv.planes, *rest, _raw_stream(at)), "attention_shared")
         self.launches += 1
 
     # ------------------------------------------------------------------ pages
@@ -921,7 +947,7 @@ class Kernels:
         n = plan.shape[0]
         if n == 0 or storage.numel() == 0:
             return
-        if not self._admit("copy_pages", 2.0 * layers * planes * heads * row * float(plan[:, 2].sum()) if self.profile is not None else 0): return
+        if self.profile is not None and not self._admit("copy_pages", 2.0 * layers * planes * heads * row * float(plan[:, 2].sum())): return
         self._check(self.lib.cima_copy_pages(storage.data_ptr(), layers, pages, planes * heads, size, row, plan.data_ptr(), n, self._stream()), "copy_pages")
         self.launches += (n - 1) // 320
 
@@ -1806,13 +1832,16 @@ class Kernels:
     def token_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, out: torch.Tensor) -> None:
         """out[i] = log softmax(logits[i])[tokens[i]] in float32.  A row with a NaN or +inf, or of nothing but -inf, gives NaN, and so does a token
         outside the vocabulary."""
-        self._need(logits, "logits", torch.float32, 2); self._need(tokens, "tokens", torch.int32, 1); self._need(out, "out", torch.float32, 1)
-        self._here(logits, tokens, out)
+        at = torch.cuda.current_device()
+        if not (logits.dtype is out.dtype is torch.float32 and tokens.dtype is torch.int32 and logits.is_contiguous() and tokens.is_contiguous() and out.is_contiguous()
+                and logits.get_device() == tokens.get_device() == out.get_device() == at and logits.dim() == 2):
+            self._need(logits, "logits", torch.float32, 2); self._need(tokens, "tokens", torch.int32, 1); self._need(out, "out", torch.float32, 1)
+            self._here(logits, tokens, out)
         n, V = logits.shape
         if tokens.numel() != n or out.numel() != n:
             raise KernelError(f"token_logprobs: {tokens.numel()} tokens and {out.numel()} places for {n} rows")
-        if not self._admit("token_logprobs", n * V * 4): return
-        self._check(self.lib.cima_token_logprobs(logits.data_ptr(), n, V, tokens.data_ptr(), out.data_ptr(), self._stream()), "token_logprobs")
+        if self.profile is not None and not self._admit("token_logprobs", n * V * 4): return
+        self._check(self.lib.cima_token_logprobs(logits.data_ptr(), n, V, tokens.data_ptr(), out.data_ptr(), _raw_stream(at)), "token_logprobs")
 
     def sample(self, logits: torch.Tensor, row_slot: torch.Tensor, params: torch.Tensor, rng: torch.Tensor,
                ring: torch.Tensor, count: torch.Tensor, work: torch.Tensor, tokens: torch.Tensor,

@@ -110,5 +110,5 @@ def logprob_reference(x, t):
     out = torch.log_softmax(x, 1).gather(1, t.long()[:, None])[:, 0]
     far = torch.where(p > 0, p * (m - x), 0.0).sum(1)
     lse = torch.logsumexp(x - m, 1)
-    bound = far * 2.0 ** -22 + (x.shape[1] / 4096 + 48) * 2.0 ** -24 + lse.abs() * 2.0 ** -22 + out.abs() * 2.0 ** -23 + (m - x.gather(1, t.long()[:, None]))[:, 0] * 2.0 ** -24
+    bound = far * 2.0 ** -22 + (x.shape[1] / 1024 + 48) * 2.0 ** -24 + lse.abs() * 2.0 ** -22 + out.abs() * 2.0 ** -23 + (m - x.gather(1, t.long()[:, None]))[:, 0] * 2.0 ** -24
     return out, bound

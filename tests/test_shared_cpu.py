@@ -10,7 +10,7 @@ def lib():
     lib = ctypes.CDLL(library_path(build=True, verbose=False))
     lib.cima_last_error.restype = ctypes.c_char_p
     from cima_b200.kernels import _SIGNATURES
-    for name in ("cima_copy_pages", "cima_attention_shared", "cima_token_logprobs"):
+    for name in ("cima_copy_pages", "cima_attention_shared", "cima_attention_shared_tc", "cima_token_logprobs"):
         getattr(lib, name).argtypes = _SIGNATURES[name]
         getattr(lib, name).restype = ctypes.c_int
     return lib
@@ -58,5 +58,19 @@ def test_bad_arguments_of_shared_attention(lib, args, word):
     a = dict(dtype=1, ld=512, cache=BASE, page=64, planes=2, groups=1, most=2, scratch=BASE, ps=2, os=2, nh=4, nkv=2, hd=64, gate=0) | args
     code = lib.cima_attention_shared(BASE, a["dtype"], a["ld"], a["cache"], BASE, 8, a["page"], a["planes"], BASE, BASE, BASE, BASE, BASE, a["groups"], a["most"],
                                      a["scratch"], BASE, a["ps"], a["os"], BASE, 256, 2, a["nh"], a["nkv"], a["hd"], 0.125, 0.0, None, a["gate"], None, 0, None)
+    assert code < 0
+    assert word in lib.cima_last_error().decode()
+
+
+@pytest.mark.parametrize("args, word", [
+    (dict(planes=3), "planes"), (dict(page=32), "page size"), (dict(nh=5), "multiple"), (dict(groups=3), "groups"), (dict(ps=0), "splits"), (dict(scratch=None), "scratch"),
+    (dict(gate=300), "gate"), (dict(cache=BASE + 8), "aligned"), (dict(hd=96), "head_dim"), (dict(ld=516), "aligned"), (dict(pages=0), "pages"),
+    (dict(pages=1 << 24), "pages"), (dict(flag=None), "error flag"),
+])
+def test_bad_arguments_of_shared_attention_on_tcgen05(lib, args, word):
+    a = dict(ld=512, cache=BASE, pages=9, page=64, planes=2, groups=1, most=2, scratch=BASE, ps=2, os=2, nh=4, nkv=2, hd=64, gate=0, flag=BASE) | args
+    code = lib.cima_attention_shared_tc(BASE, a["ld"], a["cache"], a["pages"], BASE, 8, a["page"], a["planes"], BASE, BASE, BASE, BASE, BASE, a["groups"], a["most"],
+                                        a["scratch"], BASE, a["ps"], a["os"], BASE, 256, 2, a["nh"], a["nkv"], a["hd"], 0.125, 0.0, None, a["gate"], None, 0,
+                                        a["flag"], None)
     assert code < 0
     assert word in lib.cima_last_error().decode()

@@ -80,6 +80,30 @@ def test_shared_attention_splits(K, splits, dtype):
     check(run_shared(K, c, splits=splits), *shared_reference(c))
 
 
+TC_SIZES = [([2], [1], [1], [], 1, 1, 64), ([8], [32], [1, 63, 64, 65, 100], [], 28, 4, 128), ([2, 5, 19], [1, 4, 2], [1, 2, 130, 64], [5], 12, 2, 128),
+            ([70], [9], [1, 200, 64], [], 28, 4, 128), ([33], [7], [5, 64], [900], 40, 2, 64), ([128], [3], [1], [], 8, 8, 64), ([129], [2], [7], [], 8, 8, 128)]
+
+
+@pytest.mark.parametrize("planes", [2, 1])
+@pytest.mark.parametrize("size", TC_SIZES, ids=[str(i) for i in range(len(TC_SIZES))])
+@pytest.mark.parametrize("splits", [None, (1, 1), (7, 3)])
+def test_shared_attention_on_tcgen05(K, size, planes, splits):
+    counts, prefix, own, alone, heads, kv, hd = size
+    c = shared_case(counts, prefix, own, heads, kv, hd, torch.bfloat16, planes=planes, alone=alone, seed=len(counts) + heads)
+    check(run_shared(K, c, splits=splits, tc=True), *shared_reference(c))
+    assert K.device_errors() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_shared_attention_forms_on_tcgen05(K, hd):
+    c = shared_case([26, 2], [3, 1], [1, 64, 90], 14, 2, hd, torch.bfloat16, alone=[70], gate=True, seed=11)
+    more = dict(head_sink=c.sink, slopes=c.slopes, gate_col=c.gate_col)
+    check(run_shared(K, c, tc=True, **more), *shared_reference(c, **more))
+    check(run_shared(K, c, tc=True, sink=3.0), *shared_reference(c, sink=3.0))
+    c.storage[:, 0] *= 20.0                               # scores of some hundred: the reference point moves often
+    check(run_shared(K, c, tc=True), *shared_reference(c))
+
+
 def test_shared_attention_large_scores(K):
     """Scores of several hundred, of both signs: the parts' maxima lie far from one another and a part's weight may vanish."""
     c = shared_case([4], [4], [70, 3], 8, 2, 64, torch.float32, seed=9)
@@ -146,6 +170,7 @@ def test_shared_attention_refusals(K):
                      (dict(slot=c.slot.long()), "expected"), (dict(slot=c.slot[:1]), "entries"), (dict(splits=(0, 1)), "splits"), (dict(splits=(64, 65)), "splits"),
                      (dict(shared=SharedPrefixes(c.order, c.own_page, c.groups, 5)), "groups"), (dict(gate_col=c.qkv.shape[1] - 8), "gate"),
                      (dict(shared=SharedPrefixes(c.order.cpu(), c.own_page, c.groups, 2)), "GPU tensors"), (dict(heads=3, out=out[:, :192].contiguous()), "multiple"),
+                     (dict(heads=3, out=out[:, :192].contiguous(), tc=True), "multiple"), (dict(splits=(64, 65), tc=True), "splits"),
                      (dict(kv=LayerKV(c.storage.half(), c.table, PAGE, 0, 0, 0)), "expected"), (dict(slopes=c.slopes[:2]), "slopes"),
                      (dict(shared=SharedPrefixes(c.order, c.own_page, c.groups[:, :2].contiguous(), 2)), "groups")]:
         with pytest.raises(KernelError, match=word):
