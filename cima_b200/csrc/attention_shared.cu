@@ -21,9 +21,8 @@ namespace {
 template <int HD, int PLANES, int RW, int PRE>
 __global__ void __launch_bounds__(WARPS * 32)
 k_attention_shared(const __grid_constant__ SharedArgs a) {
-  if (!a.early) cima_pdl_wait();
+  if (!a.early) wait_then_let_next();
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  cima_pdl_trigger();                                  // (the merge behind this kernel may be placed when its last block has begun; it waits for the end)
   Task t;
   if (!find_task(a, PRE > 0 ? 8 * PRE : 16 * RW, t)) return;
   if constexpr (PRE > 0) {
@@ -45,8 +44,7 @@ template <int HDP> struct F32Smem {
 template <int HDP>
 __global__ void __launch_bounds__(F_THREADS)
 k_attention_shared_f32(const __grid_constant__ SharedArgs a, int hd) {
-  cima_pdl_wait();
-  cima_pdl_trigger();
+  wait_then_let_next();
   extern __shared__ __align__(16) float sf[];
   constexpr int PITCH = F32Smem<HDP>::PITCH, PP = F32Smem<HDP>::PP, RT = F_ROWS / 16, ND = HDP / 8;
   float *sq = sf, *sk = sq + F_ROWS * PITCH, *sv = sk + PS * PITCH, *sp = sv + PS * PITCH;

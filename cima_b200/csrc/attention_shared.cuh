@@ -45,6 +45,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // The 128 threads that walk (a block may have more warps, which have no part in it).
 __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
+// The wait on the kernel before this one, and from then on the one behind may be placed beside this one's blocks, where it waits in turn.  (Not before:
+// a kernel that begins may take it that all but the one just before it are complete.)
+__device__ __forceinline__ void wait_then_let_next() {
+  cima_pdl_wait();
+  cima_pdl_trigger();
+}
+
 struct SharedArgs {
   const void* qkv;                // [B, ld]: queries (and, from gate_col on, gates) of each sequence's new position
   const void* cache;              // a layer's pages [pages, planes, kv heads, 64, head_dim]
@@ -177,7 +184,7 @@ __device__ __forceinline__ void walk(const SharedArgs& a, const Task& tk, unsign
       cp_async_commit();
       ahead++;
     }
-    cima_pdl_wait();
+    wait_then_let_next();
   }
   for (; ahead < STAGES - 1; ahead++) {
     if (p0 + ahead < p1) issue(page_of(p0 + ahead), ahead);
@@ -455,7 +462,7 @@ __device__ __forceinline__ void walk_near(const SharedArgs& a, const Task& tk, u
     load(kf, src, c, 0, newest, false);
     load(vf, src + v_off, c, 0, newest, false);
   }
-  if (a.early) cima_pdl_wait();
+  if (a.early) wait_then_let_next();
   float o[NB][HD / 16][4], mr[NB][2], lr[NB][2];
 #pragma unroll
   for (int n = 0; n < NB; n++) {
@@ -570,16 +577,15 @@ constexpr int COMBINE_WARPS = 4;
 template <typename T>
 __global__ void __launch_bounds__(32 * COMBINE_WARPS)
 k_shared_combine(const __grid_constant__ SharedArgs a, int hd) {
-  cima_pdl_trigger();
   __shared__ float4 sums[COMBINE_WARPS][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x;
   const int b = row / a.nh, h = row - b * a.nh, parts = a.prefix_splits + a.own_splits;
   const size_t base = (size_t)row * parts;
-  if (!a.early) cima_pdl_wait();
+  if (!a.early) wait_then_let_next();
   const int own = a.own_page[b];
   const int np = live_splits(own, a.prefix_splits, a.least), nr = live_splits(pages_of(a.seq_len[b]) - own, a.own_splits, a.least);
   const float extra = a.head_sink ? expf(a.head_sink[h]) : a.sink;
-  if (a.early) cima_pdl_wait();
+  if (a.early) wait_then_let_next();
   float w[MAX_PARTS / 32], l[MAX_PARTS / 32], M = -INFINITY, L = 0.f;
 #pragma unroll
   for (int i = 0; i < MAX_PARTS / 32; i++) {

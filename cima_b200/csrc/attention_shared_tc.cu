@@ -132,7 +132,7 @@ __device__ __forceinline__ void prefix_tc(const CUtensorMap* map, const SharedAr
     }
   } else {
     // ---------------------------------------------------------------- the rows
-    if (a.early) cima_pdl_wait();
+    if (a.early) wait_then_let_next();
     const __nv_bfloat16* qkv = (const __nv_bfloat16*)a.qkv;
     {                                                          // Q: chunk c of 16 bytes of a 128-byte row lies at place c ^ (row & 7); all loads at once
       constexpr int CPR = HD / 8;
@@ -287,7 +287,7 @@ __device__ __forceinline__ void own_tma(const CUtensorMap* map, const SharedArgs
       }
     }
   } else if (warp < 4) {
-    if (a.early) cima_pdl_wait();
+    if (a.early) wait_then_let_next();
     uint4 q[NB][HD / 32] = {};
     float sl2[NB][2] = {};
     int last_key[NB][2] = {};
@@ -402,9 +402,8 @@ __device__ __forceinline__ void own_tma(const CUtensorMap* map, const SharedArgs
 template <int HD, int PLANES, int OWN>
 __global__ void __launch_bounds__(TC_THREADS, 2)
 k_attention_shared_tc(const __grid_constant__ CUtensorMap map, const __grid_constant__ SharedArgs a, int* error_flag) {
-  if (!a.early) cima_pdl_wait();
+  if (!a.early) wait_then_let_next();
   extern __shared__ __align__(1024) unsigned char smem[];
-  cima_pdl_trigger();
   // An SM takes no second block of a kernel that allocates tensor memory until the first one has given up its permit to do so: so every block with
   // work does that early, those of the sequences' own pages too (without, they ran one an SM, and a prefix's second block came 1.9 us late).
   constexpr size_t SMEM = tc_smem<HD>();

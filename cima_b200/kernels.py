@@ -8,6 +8,7 @@ built or loaded, ``Kernels()`` raises.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -120,6 +121,7 @@ def extend_splits(blocks: int, max_len: int, window: int, keep_first: int) -> in
 SHARED_TC_ROWS = 16         # query rows a kv head of the largest group, above which prefixes run on tcgen05 (blocks of 128 rows)
 
 
+@lru_cache(maxsize=4096)
 def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_heads: int, max_len: int, rows: int = 128) -> Tuple[int, int]:
     """(splits of a group's prefix, splits of a sequence's own pages) of ``Kernels.attention_shared``; the kernel leaves those without work that would have
     less than two pages (on tcgen05; else one), but a block without work still has to be placed.  ``rows``: query rows of a block of a prefix.  Prefixes: one wave of blocks (two
@@ -240,6 +242,7 @@ _SIGNATURES = {
 }
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
@@ -310,7 +313,7 @@ class Kernels:
     @staticmethod
     def _here(*tensors: torch.Tensor) -> None:
         """The tensors lie on the current device, whose stream the kernel goes to."""
-        at = torch.cuda.current_device()
+        at = _current_device()
         for t in tensors:
             if t.get_device() != at:
                 raise KernelError(f"a tensor on {t.device} while cuda:{at} is the current device")
@@ -887,50 +890,56 @@ class Kernels:
         (multiples of 4) up to 128, pages of 64, every key visible; ``max_len``: positions of the longest sequence (0: not known; it bounds the
         splits); ``tc``: the prefixes on tcgen05 (None: where that is possible and there are rows for it); the other arguments are ``attention_decode``'s."""
         storage, table, order, own_page, groups = kv.storage, kv.block_table, shared.order, shared.own_page, shared.groups
-        (B, ld), dtype, at = qkv.shape, qkv.dtype, torch.cuda.current_device()
+        dtype, i32, at = qkv.dtype, torch.int32, _current_device()
         # (one glance at what is right of nearly every call; what is wrong is then named.  The host's time is most of a small step's.)
-        ints = (table, seq_slot, seq_len, order, own_page, groups)
-        if not (all([t.dtype is torch.int32 and t.is_contiguous() and t.get_device() == at for t in ints])
-                and all([t.dtype is dtype and t.is_contiguous() and t.get_device() == at for t in (qkv, out, storage)])
-                and storage.dim() == 5 and table.dim() == 2 and groups.dim() == 2):
+        if not (table.dtype is i32 and seq_slot.dtype is i32 and seq_len.dtype is i32 and order.dtype is i32 and own_page.dtype is i32 and groups.dtype is i32
+                and out.dtype is dtype and storage.dtype is dtype and qkv.is_contiguous() and out.is_contiguous() and storage.is_contiguous() and table.is_contiguous()
+                and seq_slot.is_contiguous() and seq_len.is_contiguous() and order.is_contiguous() and own_page.is_contiguous() and groups.is_contiguous()
+                and qkv.get_device() == out.get_device() == storage.get_device() == table.get_device() == seq_slot.get_device() == seq_len.get_device()
+                == order.get_device() == own_page.get_device() == groups.get_device() == at
+                and qkv.dim() == 2 and storage.dim() == 5 and table.dim() == 2 and groups.dim() == 2):
             self._need(qkv, "qkv", None, 2); self._need(out, "out", dtype, 2); self._need(storage, "cache", dtype, 5)
             for n, t, d in (("block_table", table, 2), ("seq_slot", seq_slot, 1), ("seq_len", seq_len, 1), ("order", order, 1), ("own_page", own_page, 1), ("groups", groups, 2)):
                 self._need(t, n, torch.int32, d)
-            self._here(qkv, out, storage, *ints)
-        if min(seq_slot.numel(), seq_len.numel(), order.numel(), own_page.numel()) < B:
+            self._here(qkv, out, storage, table, seq_slot, seq_len, order, own_page, groups)
+        B, ld = qkv.shape
+        if seq_slot.numel() < B or seq_len.numel() < B or order.numel() < B or own_page.numel() < B:
             raise KernelError(f"attention_shared: slots, lengths, order or own pages have fewer entries than the {B} sequences")
         if head_sink is not None or slopes is not None:
             self._need_head_sink(head_sink, n_heads, slopes)
             self._here(*[t for t in (head_sink, slopes) if t is not None])
         if kv.ring_pages or kv.window:
             raise KernelError("attention_shared: a layer with a window keeps no prefix to share")
-        pages, *page = storage.shape
-        if out.shape != (B, n_heads * head_dim) or page != [kv.planes, n_kv_heads, kv.page_size, head_dim]:
+        planes, size = kv.planes, kv.page_size
+        pages, planes_, heads_, size_, dim_ = storage.shape
+        rows, width = out.shape
+        if rows != B or width != n_heads * head_dim or planes_ != planes or heads_ != n_kv_heads or size_ != size or dim_ != head_dim:
             raise KernelError(f"attention_shared: out {tuple(out.shape)} or cache pages {tuple(storage.shape)} do not fit {B} rows of {n_heads} heads of {head_dim}")
         n_groups, three = groups.shape
-        if three != 3 or ld < n_heads * head_dim:
+        if three != 3 or ld < width:
             raise KernelError(f"attention_shared: groups {tuple(groups.shape)} are not [groups, 3], or rows of {ld} hold no {n_heads} heads of {head_dim}")
         most = shared.most
+        q = qkv.data_ptr()
         if tc is None:                                    # (the flag of the bounded waits lies on the device that first asked for it)
-            tc = (most * (n_heads // n_kv_heads) > SHARED_TC_ROWS and dtype is torch.bfloat16 and head_dim in (64, 128) and ld % 8 == 0
-                  and qkv.data_ptr() % 16 == 0 and pages * kv.planes * n_kv_heads * kv.page_size < 2 ** 31 and self.error_flag(qkv.device).get_device() == at)
+            tc = (most * n_heads > SHARED_TC_ROWS * n_kv_heads and dtype is torch.bfloat16 and head_dim in (64, 128) and ld % 8 == 0 and q % 16 == 0
+                  and pages * planes * n_kv_heads * size < 2 ** 31 and self.error_flag(qkv.device).get_device() == at)
         elif tc and dtype is not torch.bfloat16:
             raise KernelError(f"attention_shared: {dtype} on tcgen05; it takes bfloat16")
         np_, no = splits or shared_splits(n_groups, most, B, n_heads, n_kv_heads, max_len, 128 if tc else 32 if dtype is torch.float32 else 16)
-        if self.profile is not None and not self._admit(f"attention_shared[{np_} + {no} splits]", *self._attention_work(qkv, n_heads, n_kv_heads, head_dim, kv.planes)): return
+        if self.profile is not None and not self._admit(f"attention_shared[{np_} + {no} splits]", *self._attention_work(qkv, n_heads, n_kv_heads, head_dim, planes)): return
         # this call's own, as attention_decode's
         cells = B * n_heads * (np_ + no)
-        part = torch.empty(cells * (head_dim + 2), dtype=torch.float32, device=qkv.device).data_ptr()
-        rest = (seq_slot.data_ptr(), seq_len.data_ptr(), order.data_ptr(), own_page.data_ptr(), groups.data_ptr(), n_groups, most, part, part + 4 * cells * head_dim,
-                np_, no, out.data_ptr(), out.shape[1], B, n_heads, n_kv_heads, head_dim, scale, sink, _ptr(head_sink), gate_col, _ptr(slopes), int(early))
+        part = qkv.new_empty(cells * (head_dim + 2), dtype=torch.float32).data_ptr()
+        rest = (table.data_ptr(), table.shape[1], size, planes, seq_slot.data_ptr(), seq_len.data_ptr(), order.data_ptr(), own_page.data_ptr(), groups.data_ptr(),
+                n_groups, most, part, part + 4 * cells * head_dim, np_, no, out.data_ptr(), width, B, n_heads, n_kv_heads, head_dim, scale, sink,
+                None if head_sink is None else head_sink.data_ptr(), gate_col, None if slopes is None else slopes.data_ptr(), 1 if early else 0)
         if tc:
             flag = self.error_flag(qkv.device)
             self._here(flag)
-            self._check(self.lib.cima_attention_shared_tc(qkv.data_ptr(), ld, storage.data_ptr(), pages, table.data_ptr(), table.shape[1], kv.page_size, kv.planes,
-                                                          *rest, flag.data_ptr(), _raw_stream(at)), "attention_shared_tc")
+            self._check(self.lib.cima_attention_shared_tc(q, ld, storage.data_ptr(), pages, *rest, flag.data_ptr(), _raw_stream(at)), "attention_shared_tc")
         else:
-            self._check(self.lib.cima_attention_shared(qkv.data_ptr(), F32 if dtype is torch.float32 else dtype_code(dtype), ld, storage.data_ptr(), table.data_ptr(),
-                                                       table.shape[1], kv.page_size, kv.planes, *rest, _raw_stream(at)), "attention_shared")
+            self._check(self.lib.cima_attention_shared(q, F32 if dtype is torch.float32 else dtype_code(dtype), ld, storage.data_ptr(), *rest, _raw_stream(at)),
+                        "attention_shared")
         self.launches += 1
 
     # ------------------------------------------------------------------ pages
@@ -1832,7 +1841,7 @@ class Kernels:
     def token_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, out: torch.Tensor) -> None:
         """out[i] = log softmax(logits[i])[tokens[i]] in float32.  A row with a NaN or +inf, or of nothing but -inf, gives NaN, and so does a token
         outside the vocabulary."""
-        at = torch.cuda.current_device()
+        at = _current_device()
         if not (logits.dtype is out.dtype is torch.float32 and tokens.dtype is torch.int32 and logits.is_contiguous() and tokens.is_contiguous() and out.is_contiguous()
                 and logits.get_device() == tokens.get_device() == out.get_device() == at and logits.dim() == 2):
             self._need(logits, "logits", torch.float32, 2); self._need(tokens, "tokens", torch.int32, 1); self._need(out, "out", torch.float32, 1)

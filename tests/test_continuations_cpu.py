@@ -359,3 +359,14 @@ def test_steps_of_forks_are_their_own():
             assert torch.allclose(row, plain_forward(W, cfg, hist[s]).float()[-1], atol=2e-4, rtol=1e-4)
     c.close(list(hist))
     c.check()
+
+
+def test_prefixes_are_read_once_where_that_is_worth_it():
+    from cima_b200.engine.model import worth_sharing
+    page = 2 * 4 * 64 * 128 * 2                           # the 7B shape's, bfloat16
+    group = lambda n, pages: [(list(range(n)), pages)]   # noqa: E731
+    for n, no, yes in ((4, 16, 32), (8, 10, 32), (48, 4, 8)):
+        assert not worth_sharing(group(n, no), n, page, False) and worth_sharing(group(n, yes), n, page, False)
+    small = 2 * 2 * 64 * 64 * 4
+    assert not worth_sharing(group(2, 1), 2, small, True) and worth_sharing(group(2, 4), 2, small, True)
+    assert not worth_sharing([], 8, page, False)

@@ -24,6 +24,13 @@ def lm_of(shape, dtype, **kw):
     return cima_b200.LM(_models[key], **kw)
 
 
+@pytest.fixture
+def always(monkeypatch):
+    """Prefixes are read once however short they are (of these tiny models none would be long enough)."""
+    from cima_b200.engine import model
+    monkeypatch.setattr(model, "worth_sharing", lambda groups, *a: bool(groups))
+
+
 def tokens(V, n, seed):
     return [random.Random(seed).randrange(V) for _ in range(1)] + [random.Random(seed * 1000 + i).randrange(V) for i in range(n - 1)]
 
@@ -34,7 +41,7 @@ SMALL = ["tiny-b", "vunovik-tiny", "gisirax-tiny", "lipizen-tiny", "netezen-tiny
 @pytest.mark.parametrize("shape", SMALL)
 @pytest.mark.parametrize("pipeline", [True, False])
 @pytest.mark.parametrize("opts", [dict(temperature=0, repeat_penalty=1.0), dict(temperature=0.9, top_k=30, seed=9)], ids=["greedy", "sampled"])
-def test_continuations_are_what_single_answers_would_be(shape, pipeline, opts):
+def test_continuations_are_what_single_answers_would_be(shape, pipeline, opts, always):
     """32-bit, every architecture (recurrences whose state is copied, rings of windows, layers that read another's keys): each continuation has the
     tokens of a request of its own."""
     lm = lm_of(shape, "float32", pipeline=pipeline)
@@ -57,7 +64,7 @@ def test_continuations_are_what_single_answers_would_be(shape, pipeline, opts):
 @pytest.mark.parametrize("dtype, near", [("float32", 2e-4), ("bfloat16", 4e-2)])
 @pytest.mark.parametrize("shape", ["tiny-b", "vunovik-tiny", "pelatar-tiny", "gudarax-tiny"])
 @pytest.mark.parametrize("graphs", [True, False])
-def test_steps_of_forks_beside_sequences_of_their_own(shape, dtype, near, graphs):
+def test_steps_of_forks_beside_sequences_of_their_own(shape, dtype, near, graphs, always):
     """Teacher-forced steps of forks, and of the same tokens as sequences that share nothing: the logits agree within what the precision's
     steps may differ from the plain implementation's.  Forks of forks, a rewound one, steps of some of them, other orders."""
     lm = lm_of(shape, dtype, use_graphs=graphs)
@@ -104,7 +111,7 @@ def test_steps_of_forks_beside_sequences_of_their_own(shape, dtype, near, graphs
     lm.model.check_device()
 
 
-def test_shared_attention_is_what_runs(monkeypatch):
+def test_shared_attention_is_what_runs(monkeypatch, always):
     """A decoding step of continuations with whole pages in common takes the shared kernel, recorded; one without does not."""
     lm = lm_of("tiny-b", "bfloat16", pipeline=False)
     K, calls = lm.model.rt.kernels, []
@@ -117,7 +124,7 @@ def test_shared_attention_is_what_runs(monkeypatch):
     assert not calls
 
 
-def test_bfloat16_continuations_choose_near_maxima():
+def test_bfloat16_continuations_choose_near_maxima(always):
     """Greedy continuations in bfloat16 equal one another, token by token (their rows hold the same numbers), and so do their log-probabilities."""
     lm = lm_of("tiny-b", "bfloat16")
     got = lm.generate([tokens(1000, 150, 8)], max_tokens=30, temperature=0, repeat_penalty=1.0, ignore_eos=True, continuations=5, logprobs=True)
@@ -138,7 +145,7 @@ def test_scores_in_pieces(dtype):
         assert lm.score([seq, seq[:3]], rows=rows)[0] == pytest.approx(want, abs=1e-3 if dtype == "float32" else 4e-2)
 
 
-def test_kept_continuations_and_a_later_turn():
+def test_kept_continuations_and_a_later_turn(always):
     """Kept sequences that share their prompt's pages: the next turn of each goes on from its own, the others' pages stay what they were."""
     lm = lm_of("tiny-b", "float32", retain=4)
     plain = lm_of("tiny-b", "float32")
@@ -154,7 +161,7 @@ def test_kept_continuations_and_a_later_turn():
     lm.model.cache.check()
 
 
-def test_two_models_caches_on_two_streams():
+def test_two_models_caches_on_two_streams(always):
     """Forks of one cache stepped on a side stream while another cache's run on the current one: the results are those of one after the other."""
     lms = [lm_of("tiny-b", "float32"), lm_of("vunovik-tiny", "float32")]
     want = []
@@ -168,6 +175,39 @@ def test_two_models_caches_on_two_streams():
     torch.cuda.synchronize()
     assert [r.tokens for r in got] == [r.tokens for r in want[0]] and [r.tokens for r in other] == [r.tokens for r in want[1]]
     c.check()
+
+
+def test_wide_heads_and_long_prompts_choose_for_themselves(monkeypatch):
+    """A model of the 7B shape's heads (two narrow layers): continuations of a long prompt read it once, recorded and issued, and their logits are those of
+    sequences that share nothing; a short prompt's do not."""
+    cfg = dict(model_type="qwen2", architectures=["Qwen2ForCausalLM"], num_hidden_layers=2, hidden_size=256, num_attention_heads=28, num_key_value_heads=4, head_dim=128,
+               intermediate_size=256, vocab_size=512, rope_theta=1e4, rms_norm_eps=1e-6, tie_word_embeddings=True, max_position_embeddings=8192)
+    for graphs in (True, False):
+        lm = cima_b200.load(config=cfg, seed=1, dtype="bfloat16", max_tokens=64 * 700, verbose=False, use_graphs=graphs)
+        c, K, calls = lm.model.cache, lm.model.rt.kernels, []
+        whole = K.attention_shared
+        monkeypatch.setattr(K, "attention_shared", lambda *a, **kw: (calls.append(a[4].most), whole(*a, **kw))[1])
+        for n, shares in ((4100, True), (200, False)):
+            calls.clear()
+            base = tokens(512, n, 5)
+            a, = c.open(1)
+            lm.step([StepEntry(a, base)])
+            slots = [a] + c.fork(a, 7)
+            hist = [list(base) for _ in slots]
+            for step in range(5):
+                new = [(7 * i + step) % 512 for i in range(8)]
+                got = lm.step([StepEntry(s, [t], [0]) for s, t in zip(slots, new)])
+                for h, t in zip(hist, new):
+                    h.append(t)
+            alone = c.open(2)
+            lm.step([StepEntry(s, h[:-1]) for s, h in zip(alone, (hist[2], hist[7]))])
+            want = lm.step([StepEntry(s, [h[-1]], [0]) for s, h in zip(alone, (hist[2], hist[7]))])
+            assert (got[[2, 7]] - want).abs().max().item() <= 4e-2
+            assert (8 in calls) == shares
+            c.close(slots + alone)
+            c.check()
+        lm.model.check_device()
+        del lm
 
 
 def test_the_command_line_gives_several_answers_with_scores(capsys):
