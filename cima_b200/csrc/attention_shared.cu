@@ -33,26 +33,21 @@ k_attention_shared(const __grid_constant__ SharedArgs a) {
   }
 }
 
-// The same in float32, sums and all, by multiply-adds: a block takes ROWS rows, a page's keys lie in shared memory, a thread has RT rows x 8 keys of
-// the scores and RT rows x HDP / 8 values of the result.  hd is a multiple of 4.
+// The same in float32, sums and all, by multiply-adds: a block takes 16 RT rows, a page's keys and values lie in shared memory, a thread has RT rows x 8
+// keys of the scores and RT rows x HDP / 8 values of the result, so that what it reads of a page serves RT rows at once.  hd is a multiple of 4.
 constexpr int F_THREADS = 128, F_ROWS = 32;
 template <int HDP> struct F32Smem {
   static constexpr int PITCH = HDP + 4, PP = PS + 4;
   static constexpr size_t floats = (size_t)F_ROWS * PITCH + 2 * PS * PITCH + F_ROWS * PP;
 };
 
-template <int HDP>
-__global__ void __launch_bounds__(F_THREADS)
-k_attention_shared_f32(const __grid_constant__ SharedArgs a, int hd) {
-  wait_then_let_next();
-  extern __shared__ __align__(16) float sf[];
-  constexpr int PITCH = F32Smem<HDP>::PITCH, PP = F32Smem<HDP>::PP, RT = F_ROWS / 16, ND = HDP / 8;
+template <int HDP, int RT>
+__device__ __forceinline__ void walk_f32(const SharedArgs& a, const Task& tk, int hd, float* sf) {
+  constexpr int PITCH = F32Smem<HDP>::PITCH, PP = F32Smem<HDP>::PP, ND = HDP / 8;
   float *sq = sf, *sk = sq + F_ROWS * PITCH, *sv = sk + PS * PITCH, *sp = sv + PS * PITCH;
-  Task tk;
-  if (!find_task(a, F_ROWS, tk)) return;
   const float* cache = (const float*)a.cache;
-  const int tid = threadIdx.x, ty = tid >> 3, tx = tid & 7, len = a.seq_len[tk.seq], h4 = hd / 4;
-  for (int i = tid; i < F_ROWS * (HDP / 4); i += F_THREADS) {
+  const int tid = threadIdx.x, ty = tid >> 3, tx = tid & 7, len = tk.len, h4 = hd / 4;
+  for (int i = tid; i < 16 * RT * (HDP / 4); i += F_THREADS) {
     const int r = i / (HDP / 4), c = i % (HDP / 4);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < tk.rows && c < h4) {
@@ -68,22 +63,22 @@ k_attention_shared_f32(const __grid_constant__ SharedArgs a, int hd) {
 #pragma unroll
   for (int r = 0; r < RT; r++) {
     m[r] = -INFINITY, l[r] = 0.f, slope[r] = 0.f, last_key[r] = 0;
-    if (ty + 16 * r < tk.rows) {
+    if (a.slopes && ty + 16 * r < tk.rows) {
       int seq, head;
       row_of(a, tk, ty + 16 * r, seq, head);
       last_key[r] = a.seq_len[seq] - 1;
-      if (a.slopes) slope[r] = a.slopes[head];
+      slope[r] = a.slopes[head];
     }
 #pragma unroll
     for (int d = 0; d < ND; d++) acc[r][d] = 0.f;
   }
-  const int live_rt = (tk.rows + 15) / 16;
+  const int* table = a.pg.table + (size_t)tk.slot * a.pg.width;
   for (int p = tk.first; p < tk.last; p++) {
-    const int page = a.pg.table[(size_t)tk.slot * a.pg.width + p];
-    const float* ksrc = cache + ((size_t)page * a.pg.planes * a.nkv + tk.kvh) * (size_t)(PS * hd);
+    const float* ksrc = cache + ((size_t)table[p] * a.pg.planes * a.nkv + tk.kvh) * (size_t)(PS * hd);
     const float* vsrc = ksrc + a.pg.value_offset();
-    const int n = tk.prefix ? PS : min(PS, len - p * PS);       // positions behind the sequence's end count as zeros
+    const int n = min(PS, len - p * PS);                // positions behind the sequence's end count as zeros
     __syncthreads();
+#pragma unroll 4
     for (int i = tid; i < PS * (HDP / 4); i += F_THREADS) {
       const int r = i / (HDP / 4), c = i % (HDP / 4);
       float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
@@ -95,74 +90,93 @@ k_attention_shared_f32(const __grid_constant__ SharedArgs a, int hd) {
       *reinterpret_cast<float4*>(sv + r * PITCH + 4 * c) = vv;
     }
     __syncthreads();
+    float s[RT][8];
 #pragma unroll
-    for (int rr = 0; rr < RT; rr++) {
-      if (rr >= live_rt) break;
-      const int row = ty + 16 * rr;
-      float s[8];
+    for (int r = 0; r < RT; r++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) s[j] = 0.f;
-      for (int c = 0; c < h4; c++) {
-        const float4 qv = *reinterpret_cast<const float4*>(sq + row * PITCH + 4 * c);
+      for (int j = 0; j < 8; j++) s[r][j] = 0.f;
+    for (int c = 0; c < h4; c++) {
+      float4 q[RT];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float4 kv = *reinterpret_cast<const float4*>(sk + (tx + 8 * j) * PITCH + 4 * c);
-          s[j] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[j]))));
-        }
+      for (int r = 0; r < RT; r++) q[r] = *reinterpret_cast<const float4*>(sq + (ty + 16 * r) * PITCH + 4 * c);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float4 kv = *reinterpret_cast<const float4*>(sk + (tx + 8 * j) * PITCH + 4 * c);
+#pragma unroll
+        for (int r = 0; r < RT; r++) s[r][j] = fmaf(q[r].x, kv.x, fmaf(q[r].y, kv.y, fmaf(q[r].z, kv.z, fmaf(q[r].w, kv.w, s[r][j]))));
       }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const int key = tx + 8 * j;
-        s[j] = key < n ? fmaf(slope[rr], (float)(p * PS + key - last_key[rr]), s[j] * a.scale) : -INFINITY;
-        mx = fmaxf(mx, s[j]);
+        s[r][j] = key < n ? fmaf(slope[r], (float)(p * PS + key - last_key[r]), s[r][j] * a.scale) : -INFINITY;
+        mx = fmaxf(mx, s[r][j]);
       }
 #pragma unroll
       for (int x = 1; x < 8; x *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      const float mn = fmaxf(m[rr], mx), ref = mn == -INFINITY ? 0.f : mn, corr = expf(m[rr] - ref);
-      m[rr] = mn;
+      const float mn = fmaxf(m[r], mx), ref = mn == -INFINITY ? 0.f : mn, corr = expf(m[r] - ref);
+      m[r] = mn;
       float ps = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        s[j] = expf(s[j] - ref);
-        ps += s[j];
-        sp[row * PP + tx + 8 * j] = s[j];
+        s[r][j] = expf(s[r][j] - ref);
+        ps += s[r][j];
+        sp[(ty + 16 * r) * PP + tx + 8 * j] = s[r][j];
       }
-      l[rr] = fmaf(l[rr], corr, ps);
+      l[r] = fmaf(l[r], corr, ps);
 #pragma unroll
-      for (int d = 0; d < ND; d++) acc[rr][d] *= corr;
-      __syncwarp();                                    // a row's 8 threads are of one warp
-      for (int k = 0; k < PS; k++) {
-        const float w = sp[row * PP + k];
+      for (int d = 0; d < ND; d++) acc[r][d] *= corr;
+    }
+    __syncwarp();                                      // a row's 8 threads are of one warp
+#pragma unroll 4
+    for (int k = 0; k < PS; k++) {
+      float w[RT];
 #pragma unroll
-        for (int d = 0; d < ND; d += 4) {
-          const float4 vv = *reinterpret_cast<const float4*>(sv + k * PITCH + 4 * tx + 8 * d);
-          acc[rr][d] = fmaf(w, vv.x, acc[rr][d]);
-          acc[rr][d + 1] = fmaf(w, vv.y, acc[rr][d + 1]);
-          acc[rr][d + 2] = fmaf(w, vv.z, acc[rr][d + 2]);
-          acc[rr][d + 3] = fmaf(w, vv.w, acc[rr][d + 3]);
+      for (int r = 0; r < RT; r++) w[r] = sp[(ty + 16 * r) * PP + k];
+#pragma unroll
+      for (int d = 0; d < ND; d += 4) {
+        const float4 vv = *reinterpret_cast<const float4*>(sv + k * PITCH + 4 * tx + 8 * d);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          acc[r][d] = fmaf(w[r], vv.x, acc[r][d]);
+          acc[r][d + 1] = fmaf(w[r], vv.y, acc[r][d + 1]);
+          acc[r][d + 2] = fmaf(w[r], vv.z, acc[r][d + 2]);
+          acc[r][d + 3] = fmaf(w[r], vv.w, acc[r][d + 3]);
         }
       }
-      __syncwarp();
     }
   }
   const int parts = a.prefix_splits + a.own_splits;
 #pragma unroll
-  for (int rr = 0; rr < RT; rr++) {
-    float lt = l[rr];
+  for (int r = 0; r < RT; r++) {
+    float lt = l[r];
 #pragma unroll
     for (int x = 1; x < 8; x *= 2) lt += __shfl_xor_sync(0xffffffffu, lt, x);
-    if (ty + 16 * rr >= tk.rows) continue;
+    if (ty + 16 * r >= tk.rows) continue;
     int seq, head;
-    row_of(a, tk, ty + 16 * rr, seq, head);
+    row_of(a, tk, ty + 16 * r, seq, head);
     const size_t pi = ((size_t)seq * a.nh + head) * parts + tk.part;
 #pragma unroll
-    for (int d = 0; d < ND; d++) {
-      const int at = 4 * tx + 8 * (d & ~3) + (d & 3);
-      if (at < hd) a.part_o[pi * hd + at] = acc[rr][d];
+    for (int d = 0; d < ND; d += 4) {
+      const int at = 4 * tx + 8 * d;
+      if (at < hd) *reinterpret_cast<float4*>(a.part_o + pi * hd + at) = make_float4(acc[r][d], acc[r][d + 1], acc[r][d + 2], acc[r][d + 3]);
     }
-    if (tx == 0) { a.part_ml[pi * 2] = m[rr] * LOG2E; a.part_ml[pi * 2 + 1] = lt; }
+    if (tx == 0) { a.part_ml[pi * 2] = m[r] * LOG2E; a.part_ml[pi * 2 + 1] = lt; }
   }
+}
+
+template <int HDP>
+__global__ void __launch_bounds__(F_THREADS)
+k_attention_shared_f32(const __grid_constant__ SharedArgs a, int hd) {
+  wait_then_let_next();
+  extern __shared__ __align__(16) float sf[];
+  Task tk;
+  if (!find_task(a, F_ROWS, tk)) return;
+  if (tk.rows > 16) walk_f32<HDP, 2>(a, tk, hd, sf);
+  else walk_f32<HDP, 1>(a, tk, hd, sf);
 }
 
 template <int HD, int PLANES, int RW, int PRE>

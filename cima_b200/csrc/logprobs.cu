@@ -43,7 +43,7 @@ __device__ __forceinline__ float4 ld_stream(const float* p) {        // a row is
   return v;
 }
 
-// The blocks of a cluster (1 to 16) share a row.  A thread has four vectors of 16 bytes on their way.
+// The blocks of a cluster (1 to 16) share a row, which is read once.  A thread has four vectors of 16 bytes on their way.
 __global__ void __launch_bounds__(THREADS)
 k_token_logprobs(const float* __restrict__ logits, int V, const int* __restrict__ tokens, float* __restrict__ out) {
   cima_pdl_wait();
@@ -151,10 +151,13 @@ extern "C" int cima_token_logprobs(const float* logits, int n, int V, const int*
     const int rc = cima_launch(k_token_logprobs_short, dim3((n - 1) / WARP_ROWS + 1), dim3(32 * WARP_ROWS), (size_t)0, stream, 1, logits, n, V, tokens, out);
     return rc ? rc : cima_launch_result();
   }
-  // As many blocks a row as the GPU has room for (four of 512 threads an SM), each with work for all its threads; many rows: a block a row, whose
-  // start and end then weigh least.
+  // Blocks a row.  A cluster costs about a microsecond to place and to meet in, and its blocks must be placed together: many of them wait.
+  // Measured (us by blocks a row; V = 152,064): 1 row 10.9 / 7.6 / 5.3 / 4.3 / 3.7 for 1 / 2 / 4 / 8 / 16; 8 rows 11.3 / 7.9 / 5.6 / 4.6 / 4.7; 61 rows
+  // 17.3 / 11.9 / 9.5 / 10.9 / 14.8; 150 rows 22.3 / 19.0 / 20.7 / 22.6; 300 rows 32.0 / 37.1 / 35.1; 1,200 rows 113 / 113 / 115 / 149.  V = 32,003: 1 row
+  // 3.9 / 3.8 / 3.3 / 3.3, 100 rows 4.3 / 5.3 / 5.6 / 8.9; V = 5,001: 1 row 2.3 / 3.3.  A block has one round of loads at least.
   int C = 16;
-  while (C > 1 && ((long long)n * C > 592 || V / C < 4 * THREADS)) C /= 2;
+  for (; C > 1; C /= 2)
+    if (V / C >= (n <= 64 ? 7500 : 16384) && (long long)n * C <= (C == 16 ? 64 : C == 8 ? 128 : C == 4 ? 400 : 300)) break;
   if (C == 16 && !wide_clusters()) C = 8;
   for (int i = 0; i < n; i += 65535) {
     const int m = n - i < 65535 ? n - i : 65535;

@@ -125,7 +125,7 @@ SHARED_TC_ROWS = 16         # query rows a kv head of the largest group, above w
 def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_heads: int, max_len: int, rows: int = 128) -> Tuple[int, int]:
     """(splits of a group's prefix, splits of a sequence's own pages) of ``Kernels.attention_shared``; the kernel leaves those without work that would have
     less than two pages (on tcgen05; else one), but a block without work still has to be placed.  ``rows``: query rows of a block of a prefix.  Prefixes: one wave of blocks (two
-    an SM).  Own pages, of which there mostly are few: some 64 blocks, at least one a sequence and kv head; where sequences share nothing (there are more
+    an SM) at most, of four pages beyond some 96 blocks.  Own pages, of which there mostly are few: some 64 blocks, at least one a sequence and kv head; where sequences share nothing (there are more
     than the groups can hold) theirs are as long as the longest, and a block should have about 8 of them, in four waves at most."""
     group, pages = n_heads // n_kv_heads, (max_len + 63) // 64 if max_len > 0 else 1 << 16
     prefix = n_groups * -(-most * group // rows) * n_kv_heads
@@ -134,7 +134,9 @@ def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_head
     if n_seqs > n_groups * most:
         own = max(own, min(16, pages // 8, 4 * SPLIT_BLOCKS // blocks))
     least = 2 if rows == 128 else 1
-    return max(1, min(48, SPLIT_BLOCKS // max(1, prefix), pages // least)), max(1, min(own, pages // least))
+    if rows == 32:                                     # (float32: a page is long work, and blocks are small)
+        return max(1, min(96, 2 * SPLIT_BLOCKS // max(1, prefix), pages)), max(1, min(32, max(own, SPLIT_BLOCKS // blocks), pages))
+    return max(1, min(48, SPLIT_BLOCKS // max(1, prefix), max(pages // 4, min(pages // least, 96 // max(1, prefix))))), max(1, min(own, pages // least))
 
 
 # epilogues of the skinny product
