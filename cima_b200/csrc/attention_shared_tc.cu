@@ -35,8 +35,8 @@ __device__ __forceinline__ void prefix_tc(const CUtensorMap* map, const SharedAr
   unsigned char* sv = sk + 2 * NH * KV_BLOCK;
   unsigned long long* bars = (unsigned long long*)(sv + 2 * NH * KV_BLOCK);
   unsigned long long *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *s_full = bars + 9, *p_full = bars + 11,
-                     *pv_done = bars + 13;
-  volatile int* abort_flag = (volatile int*)(bars + 14);
+                     *pv_done = bars + 13, *all_done = bars + 14;
+  volatile int* abort_flag = (volatile int*)(bars + 15);
   long long* row_at = (long long*)(bars + 16);                 // [rows] where a row's query begins, -1: no row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = tk.last - tk.first;
@@ -49,6 +49,7 @@ __device__ __forceinline__ void prefix_tc(const CUtensorMap* map, const SharedAr
       mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4);
     }
     mbar_init(pv_done, 1);
+    mbar_init(all_done, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -129,6 +130,7 @@ __device__ __forceinline__ void prefix_tc(const CUtensorMap* map, const SharedAr
         umma_commit(&v_empty[s]);
         umma_commit(pv_done);
       }
+      if (ok) umma_commit(all_done);
     }
   } else {
     // ---------------------------------------------------------------- the rows
@@ -218,9 +220,9 @@ __device__ __forceinline__ void prefix_tc(const CUtensorMap* map, const SharedAr
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[s]);                  // (one barrier a buffer: no waiter can be a phase behind)
     }
-    // a wait on a parity answers for the last phase of that parity: page n - 2 before page n - 1
-    if (ok && n > 1) ok = mbar_wait(pv_done, (n - 2) & 1, error_flag, abort_flag);
-    if (ok) ok = mbar_wait(pv_done, (n - 1) & 1, error_flag, abort_flag);
+    // The last P V has a barrier of its own: pv_done, asked by parity, would answer for page n - 3 while page n - 2 is not complete, and not
+    // at all for page n - 2 once page n - 1 is (a warp held up between its last announcement and here waited two seconds).
+    if (ok) ok = mbar_wait(all_done, 0, error_flag, abort_flag);
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // a warp's 32 rows through shared memory (in the tiles' place: every MMA that read them is complete), so that a row leaves as one piece

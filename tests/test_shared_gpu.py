@@ -94,6 +94,22 @@ def test_shared_attention_on_tcgen05(K, size, planes, splits):
     assert K.device_errors() == 0
 
 
+def test_many_launches_on_tcgen05_in_a_row(K):
+    """Some thousand launches as a recorded step makes them, each let begin while the kernel before it ends: no bounded wait runs out (one in
+    some thousand did, where a warp asked for a phase that two later ones had overtaken), and every result is the first one's."""
+    c = shared_case([48], [32], [100, 1, 64, 130], 28, 4, 128, torch.bfloat16, seed=2)
+    want = run_shared(K, c)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = [run_shared(K, c, early=True) for _ in range(40)]
+    K.device_errors()
+    for _ in range(100):
+        g.replay()
+    torch.cuda.synchronize()
+    assert K.device_errors() == 0
+    assert all(torch.equal(o, want) for o in outs)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_shared_attention_forms_on_tcgen05(K, hd):
     c = shared_case([26, 2], [3, 1], [1, 64, 90], 14, 2, hd, torch.bfloat16, alone=[70], gate=True, seed=11)
