@@ -107,7 +107,8 @@ k_attention_prefill_tc(const __grid_constant__ CUtensorMap map_qkv, const __grid
   unsigned long long* s_full = bars + 9;                       // [2]
   unsigned long long* p_full = bars + 11;                      // [2]  one per buffer of S, as s_full: see the softmax warps
   unsigned long long* pv_done = bars + 13;                     // [1]
-  unsigned* tmem_slot = (unsigned*)(bars + 14);
+  unsigned long long* all_done = bars + 14;                    // [1]  behind the last P V
+  unsigned* tmem_slot = (unsigned*)(bars + 15);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -135,6 +136,7 @@ k_attention_prefill_tc(const __grid_constant__ CUtensorMap map_qkv, const __grid
       mbar_init(&p_full[s], 4);
     }
     mbar_init(pv_done, 1);
+    mbar_init(all_done, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -229,6 +231,7 @@ k_attention_prefill_tc(const __grid_constant__ CUtensorMap map_qkv, const __grid
         umma_commit(&v_empty[s]);
         umma_commit(pv_done);
       }
+      if (ok) umma_commit(all_done);
     }
   } else {
     // ---------------------------------------------------------------- softmax: thread = query row
@@ -341,11 +344,11 @@ k_attention_prefill_tc(const __grid_constant__ CUtensorMap map_qkv, const __grid
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[s]);
     }
-    // A wait on a parity answers for the last phase of that parity.  This warp has S of tile n - 1, so P V of tile
-    // n - 3 is complete, but that of tile n - 2 need not be: asked for tile n - 1 alone, the barrier would answer for
-    // tile n - 3.  (Inside the loop a warp with S of tile j asks for tile j - 1 and cannot be answered for j - 3.)
-    if (ok && n > 1) ok = mbar_wait(pv_done, (n - 2) & 1, a.error_flag, abort_flag);
-    if (ok && n > 0) ok = mbar_wait(pv_done, (n - 1) & 1, a.error_flag, abort_flag);
+    // The last P V has a barrier of its own.  A wait on a parity answers for the last phase of that parity: pv_done, asked for tile n - 1 alone,
+    // would answer for tile n - 3 where that of n - 2 is not complete, and asked for tile n - 2 first not at all where that of n - 1 is (a warp held up
+    // between its last announcement and the question).  Inside the loop a warp with S of tile j asks for tile j - 1 and neither can be: P V of tile j
+    // waits for the warp's own announcement.
+    if (ok && n > 0) ok = mbar_wait(all_done, 0, a.error_flag, abort_flag);
     if (ok && n > 0) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const float sink = a.head_sink ? expf(a.head_sink[h]) : a.sink;
@@ -410,8 +413,8 @@ int launch_attention_tc(const void* qkv, int ld, const int* tile_seq, const int*
   else rc = make_map(&mk, qkv, T, cols, ld, BN);
   if (rc) return rc;
   constexpr int NH = HD / 64;
-  const size_t smem = NH * (size_t)HALF_BYTES + 2 * NH * (size_t)KHALF_BYTES + 2 * (size_t)HD * 128 + 14 * 8 + 16;
-  static_assert(14 * 8 + 8 <= 14 * 8 + 16, "barriers and flags fit their place");
+  const size_t smem = NH * (size_t)HALF_BYTES + 2 * NH * (size_t)KHALF_BYTES + 2 * (size_t)HD * 128 + 15 * 8 + 16;
+  static_assert(15 * 8 + 8 <= 15 * 8 + 16, "barriers and flags fit their place");
   static bool raised = false;
   if (!raised) {
     cudaError_t e = cudaFuncSetAttribute(k_attention_prefill_tc<HD, FROM_CACHE, NEAR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
