@@ -76,6 +76,7 @@ class SharedPrefixes:
     own_page: torch.Tensor       # [seqs] pages that sequence i has in common with its group (0: it is in none); its own begin there
     groups: torch.Tensor         # [groups, 3] place of the group's first sequence in ``order``, sequences, pages
     most: int                    # sequences of the largest group
+    pages: int = 0               # a bound on the pages of a group (0: not known), for the choice of splits only
 
     @staticmethod
     def pack(groups: Sequence[Tuple[Sequence[int], int]], n_seqs: int) -> np.ndarray:
@@ -91,9 +92,9 @@ class SharedPrefixes:
         return out
 
     @classmethod
-    def over(cls, packed: torch.Tensor, n_seqs: int, most: int) -> "SharedPrefixes":
+    def over(cls, packed: torch.Tensor, n_seqs: int, most: int, pages: int = 0) -> "SharedPrefixes":
         """The arrays of ``packed`` (on the device) as views."""
-        return cls(packed[:n_seqs], packed[n_seqs:2 * n_seqs], packed[2 * n_seqs:].view(-1, 3), most)
+        return cls(packed[:n_seqs], packed[n_seqs:2 * n_seqs], packed[2 * n_seqs:].view(-1, 3), most, pages)
 
 
 class KVGroup:

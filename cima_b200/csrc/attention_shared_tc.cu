@@ -21,6 +21,8 @@ using namespace cima_tc;
 constexpr int TC_ROWS = 128, TC_THREADS = 192, UMMA_K = 16;
 constexpr int Q_BLOCK = TC_ROWS * 64 * 2, KV_BLOCK = PS * 64 * 2;      // 128 rows or 64 keys of 64 dims: 128-byte rows, swizzled
 
+constexpr int FEW_ROWS = 8;
+constexpr size_t ONE_AN_SM = 120 * 1024;                       // more than half of what an SM offers
 constexpr int OWN_STAGES = 3;                                  // pages of a sequence's own on their way
 constexpr int TMEM_PREFIX = 256, TMEM_OWN = 32;               // columns of tensor memory: two buffers of S and O; the fewest there are
 // Shared memory: a prefix's Q tile, two stages of K and V, barriers and where its rows' queries lie, which is more than a sequence's own three
@@ -438,11 +440,16 @@ int launch_shared_tc(SharedArgs a, long long n_pages, int most, int* error_flag,
   a.own_rows = 8 * (G <= 8 ? 1 : WIDE);
   a.own_tiles = (G + a.own_rows - 1) / a.own_rows;
   constexpr size_t smem = tc_smem<HD>();
-  static_assert(smem >= near_smem<HD, WIDE, 4>() && smem >= OWN_STAGES * 2 * (HD / 64) * KV_BLOCK + 16 * OWN_STAGES + 32, "a sequence's own pages and their merge fit");
+  static_assert(smem <= ONE_AN_SM && smem >= near_smem<HD, WIDE, 4>() && smem >= OWN_STAGES * 2 * (HD / 64) * KV_BLOCK + 16 * OWN_STAGES + 32, "a sequence's own pages and their merge fit");
   const dim3 grid(blocks_of(a));
-  auto go = [&](auto kern, int rc) { return rc ? rc : cima_launch(kern, grid, dim3(TC_THREADS), smem, stream, 1, map, a, error_flag); };
-  const int rc = G <= 8 ? go(k_attention_shared_tc<HD, PLANES, 1>, prepare_kernel<k_attention_shared_tc<HD, PLANES, 1>>(smem))
-                        : go(k_attention_shared_tc<HD, PLANES, WIDE>, prepare_kernel<k_attention_shared_tc<HD, PLANES, WIDE>>(smem));
+  // Steps of few rows: one block an SM.  Two set the SM up for nearly all of its memory as shared memory, which it keeps while kernels follow without a
+  // pause; the products of few rows, which read their rows through L1 again and again, are 1.3 to 2 times slower then (8 sequences of the 7B shape,
+  // 2,048 / 8,192 positions in common, us a layer in the step: 50 more).  Beyond them the products are the library's, and two blocks an SM are better
+  // (48 sequences, 2,048 positions: 6 us).
+  const size_t room = a.B <= FEW_ROWS ? ONE_AN_SM : smem;
+  auto go = [&](auto kern, int rc) { return rc ? rc : cima_launch(kern, grid, dim3(TC_THREADS), room, stream, 1, map, a, error_flag); };
+  const int rc = G <= 8 ? go(k_attention_shared_tc<HD, PLANES, 1>, prepare_kernel<k_attention_shared_tc<HD, PLANES, 1>>(ONE_AN_SM))
+                        : go(k_attention_shared_tc<HD, PLANES, WIDE>, prepare_kernel<k_attention_shared_tc<HD, PLANES, WIDE>>(ONE_AN_SM));
   if (rc) return rc;
   return launch_combine<__nv_bfloat16>(a, HD, stream);
 }

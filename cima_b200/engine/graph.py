@@ -34,8 +34,9 @@ def one_token_batch(meta: torch.Tensor, n_seqs: int, max_len: int, even: bool = 
 
 
 def shared_shape(groups) -> tuple:
-    """What a recorded step of sequences that share prefixes fixes of them: (groups, sequences of the largest); () where nothing is shared."""
-    return (len(groups), max(len(members) for members, _ in groups)) if groups else ()
+    """What a recorded step of sequences that share prefixes fixes of them: (groups, sequences of the largest, pages of the longest rounded up to a power of
+    two); () where nothing is shared."""
+    return (len(groups), max(len(members) for members, _ in groups), 1 << (max(pages for _, pages in groups) - 1).bit_length()) if groups else ()
 
 
 class SharedBuffer:
@@ -45,7 +46,7 @@ class SharedBuffer:
         n = 2 * n_seqs + 3 * shape[0]
         self.n_seqs = n_seqs
         self.device = torch.zeros(n, dtype=torch.int32, device=device)
-        self.shared = SharedPrefixes.over(self.device, n_seqs, shape[1])
+        self.shared = SharedPrefixes.over(self.device, n_seqs, *shape[1:])
 
     def load(self, groups) -> None:
         host = torch.from_numpy(SharedPrefixes.pack(groups, self.n_seqs))

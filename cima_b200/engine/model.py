@@ -39,14 +39,14 @@ def parse_dtype(d) -> torch.dtype:
 
 
 def worth_sharing(groups, n_seqs: int, page_bytes: int, full_precision: bool) -> bool:
-    """Whether a one-token step's attention is the shorter for reading the groups' prefixes once: what it spares a layer (``page_bytes``: of a page of one layer)
-    against what the kernel for it takes beside the ordinary ones, which read a prefix again from L2.  Measured as us a layer, ordinary / shared, one group:
-    7B heads, 8 sequences over 1,024 / 2,048 / 4,096 positions 9.3 / 9.8, 11.6 / 10.8, 15.5 / 13.6; 48 over 256 / 512 / 2,048 13.0 / 13.7, 17.1 / 14.0,
-    38.9 / 17.9; 4 over 1,024 / 2,048 9.2 / 9.3, 11.3 / 10.4; 1.5B, 16 over 1,024 / 2,048 9.4 / 9.9, 11.5 / 10.6; 0.5B, 8 over 2,048 / 4,096 8.7 / 8.7,
-    10.7 / 9.6; 14B, 8 over 512 / 1,024 9.1 / 9.8, 11.4 / 10.6.  In float32 (0.5B) 2 sequences over 64 / 256 6.7 / 8.9, 10.6 / 9.0, 8 over 256 / 1,024 10.7 /
-    15.2, 23.0 / 17.1, 16 over 1,024 33.2 / 18.8."""
+    """Whether a one-token step's attention is the shorter for reading the groups' prefixes once: by the bytes that a layer is spared (``page_bytes``: of a page
+    of one layer), which the ordinary kernels read again from L2 in about the time that this one takes beside them where they are 70 MB.  Measured in the
+    step, 7B heads, us a layer against the ordinary kernels (MB spared): 8 sequences over 2,048 / 8,192 / 16,384 positions +1.6 (29) / -4 (117) / -15
+    (235); 4 over 16,384 -10 (101); 16 over 2,048 / 8,192 +0.7 (63) / -16 (252); 32 over 2,048 -2 (130); 48 over 448 / 2,048 +4 (43) / -17 (197).  In
+    float32 (multiply-adds, one launch after another, 0.5B heads) 2 sequences over 64 / 256 6.7 / 8.9, 10.6 / 9.0 us ordinary / shared, 8 over 256 /
+    1,024 10.7 / 15.2, 23.0 / 17.1, 16 over 1,024 33.2 / 18.8."""
     spared = page_bytes * sum((len(members) - 1) * pages for members, pages in groups)
-    return spared >= (max(0.2e6, 0.5e6 * n_seqs - 0.8e6) if full_precision else 6e6 + 0.5e6 * n_seqs)
+    return spared >= (max(0.2e6, 0.5e6 * n_seqs - 0.8e6) if full_precision else 70e6)
 
 
 def build_plan(spec: ModelSpec, rt: Optional[Runtime] = None) -> Dict[str, TensorSpec]:
@@ -302,7 +302,7 @@ class Model:
         batch = build_batch(entries, starts, self.spec.vocab, self.rt.device)
         if groups:
             packed = torch.from_numpy(SharedPrefixes.pack(groups, len(entries))).to(self.rt.device)
-            batch.shared = SharedPrefixes.over(packed, len(entries), shared_shape(groups)[1])
+            batch.shared = SharedPrefixes.over(packed, len(entries), *shared_shape(groups)[1:])
         for e, s in zip(entries, starts):
             cache.reserve(e.slot, s + len(e.tokens))
         cache.flush()
@@ -335,7 +335,7 @@ class Model:
         share then: one recorded for longer contexts serves the shorter ones too, and takes their recording's place."""
         from . import graph
         graphs = self._step_graphs
-        # (sequences that share prefixes have recordings of their own: (sequences, groups, most of a group) stands where the sequences do)
+        # (sequences that share prefixes have recordings of their own: (sequences, groups, ...) stands where the sequences do)
         key = ((len(lengths), *shape) if shape else len(lengths), self.context_bound(lengths))
         self._steps += 1
         g = graphs.get(key)

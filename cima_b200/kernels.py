@@ -122,21 +122,27 @@ SHARED_TC_ROWS = 16         # query rows a kv head of the largest group, above w
 
 
 @lru_cache(maxsize=4096)
-def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_heads: int, max_len: int, rows: int = 128) -> Tuple[int, int]:
+def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_heads: int, max_len: int, rows: int = 128, prefix_pages: int = 0) -> Tuple[int, int]:
     """(splits of a group's prefix, splits of a sequence's own pages) of ``Kernels.attention_shared``; the kernel leaves those without work that would have
-    less than two pages (on tcgen05; else one), but a block without work still has to be placed.  ``rows``: query rows of a block of a prefix.  Prefixes: one wave of blocks (two
-    an SM) at most, of four pages beyond some 96 blocks.  Own pages, of which there mostly are few: some 64 blocks, at least one a sequence and kv head; where sequences share nothing (there are more
-    than the groups can hold) theirs are as long as the longest, and a block should have about 8 of them, in four waves at most."""
+    less than two pages (on tcgen05; else one), but a block without work still has to be placed.  ``rows``: query rows of a block of a prefix, 128 on
+    tcgen05; ``prefix_pages``: a bound on a group's pages (0: none known).  Prefixes on tcgen05: some 96 blocks, for up to 8 sequences no more (one an SM then),
+    beyond them as many of four pages as one wave of two an SM holds.  Own pages, of which there mostly are few: some 64 blocks, at least one a sequence
+    and kv head; where sequences share nothing (there are more than the groups can hold) theirs are as long as the longest, and a block should have about 8
+    of them, in four waves at most."""
     group, pages = n_heads // n_kv_heads, (max_len + 63) // 64 if max_len > 0 else 1 << 16
-    prefix = n_groups * -(-most * group // rows) * n_kv_heads
+    prefix = max(1, n_groups * -(-most * group // rows) * n_kv_heads)
     blocks = n_seqs * n_kv_heads * -(-group // 16)
+    shared = min(pages, prefix_pages) if prefix_pages else pages
+    least = 2 if rows == 128 else 1
     own = min(4, 64 // blocks)
     if n_seqs > n_groups * most:
         own = max(own, min(16, pages // 8, 4 * SPLIT_BLOCKS // blocks))
-    least = 2 if rows == 128 else 1
-    if rows == 32:                                     # (float32: a page is long work, and blocks are small)
-        return max(1, min(96, 2 * SPLIT_BLOCKS // max(1, prefix), pages)), max(1, min(32, max(own, SPLIT_BLOCKS // blocks), pages))
-    return max(1, min(48, SPLIT_BLOCKS // max(1, prefix), max(pages // 4, min(pages // least, 96 // max(1, prefix))))), max(1, min(own, pages // least))
+    if rows == 32:                                     # float32: a page is long work, and blocks are small
+        return max(1, min(96, 2 * SPLIT_BLOCKS // prefix, shared)), max(1, min(32, max(own, SPLIT_BLOCKS // blocks), pages))
+    some = min(shared // least, 96 // prefix)
+    if n_seqs > 8 or rows != 128:
+        some = max(some, min(shared // 4, SPLIT_BLOCKS // prefix))
+    return max(1, min(48, some)), max(1, min(own, pages // least))
 
 
 # epilogues of the skinny product
@@ -927,7 +933,8 @@ class Kernels:
                   and pages * planes * n_kv_heads * size < 2 ** 31 and self.error_flag(qkv.device).get_device() == at)
         elif tc and dtype is not torch.bfloat16:
             raise KernelError(f"attention_shared: {dtype} on tcgen05; it takes bfloat16")
-        np_, no = splits or shared_splits(n_groups, most, B, n_heads, n_kv_heads, max_len, 128 if tc else 32 if dtype is torch.float32 else 16)
+        np_, no = splits or shared_splits(n_groups, most, B, n_heads, n_kv_heads, max_len, 128 if tc else 32 if dtype is torch.float32 else 16,
+                                           shared.pages)
         if self.profile is not None and not self._admit(f"attention_shared[{np_} + {no} splits]", *self._attention_work(qkv, n_heads, n_kv_heads, head_dim, planes)): return
         # this call's own, as attention_decode's
         cells = B * n_heads * (np_ + no)

@@ -216,6 +216,8 @@ def test_groups_of_a_step():
     assert c.shared_groups([xs[0], z, ys[0]]) == [([0, 2], 2)]
     assert c.shared_groups([xs[1], ys[0], xs[2]]) == [([0, 2], 5)]              # five pages spared; all three together would spare four
     assert c.shared_groups([z, xs[0]]) == [] and c.shared_groups([xs[0]]) == []
+    from cima_b200.engine.graph import shared_shape
+    assert shared_shape([([1, 3, 2], 5), ([4, 0], 2)]) == (2, 3, 8) and shared_shape([([0, 1], 1)]) == (1, 2, 1) and shared_shape([]) == ()
     packed = torch.from_numpy(SharedPrefixes.pack([([1, 3], 5), ([4, 0], 2)], 6))
     sp = SharedPrefixes.over(packed, 6, 2)
     assert sp.order.tolist() == [1, 3, 4, 0, 2, 5] and sp.own_page.tolist() == [2, 5, 0, 5, 2, 0] and sp.groups.tolist() == [[0, 2, 5], [2, 2, 2]]
@@ -365,7 +367,7 @@ def test_prefixes_are_read_once_where_that_is_worth_it():
     from cima_b200.engine.model import worth_sharing
     page = 2 * 4 * 64 * 128 * 2                           # the 7B shape's, bfloat16
     group = lambda n, pages: [(list(range(n)), pages)]   # noqa: E731
-    for n, no, yes in ((4, 16, 32), (8, 10, 32), (48, 4, 8)):
+    for n, no, yes in ((4, 64, 256), (8, 32, 128), (48, 7, 32)):
         assert not worth_sharing(group(n, no), n, page, False) and worth_sharing(group(n, yes), n, page, False)
     small = 2 * 2 * 64 * 64 * 4
     assert not worth_sharing(group(2, 1), 2, small, True) and worth_sharing(group(2, 4), 2, small, True)

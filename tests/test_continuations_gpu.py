@@ -187,7 +187,7 @@ def test_wide_heads_and_long_prompts_choose_for_themselves(monkeypatch):
         c, K, calls = lm.model.cache, lm.model.rt.kernels, []
         whole = K.attention_shared
         monkeypatch.setattr(K, "attention_shared", lambda *a, **kw: (calls.append(a[4].most), whole(*a, **kw))[1])
-        for n, shares in ((4100, True), (200, False)):
+        for n, shares in ((6500, True), (200, False)):
             calls.clear()
             base = tokens(512, n, 5)
             a, = c.open(1)
