@@ -466,6 +466,7 @@ extern "C" int cima_attention_shared_tc(const void* qkv, int ld, const void* cac
   if (B <= 0) return 0;
   if (hd != 64 && hd != 128) return cima_fail(CIMA_E_SIZE, "attention_shared_tc: head_dim %d; this kernel takes 64 or 128", hd);
   if (!error_flag) return cima_fail(CIMA_E_ARG, "attention_shared_tc: an error flag on the device is needed");
+  if (!(scale >= 0.f)) return cima_fail(CIMA_E_ARG, "attention_shared_tc: a scale of %g; this kernel takes the maxima of the unscaled scores and no negative one", scale);
   if (ld % 8 || ((uintptr_t)qkv & 15)) return cima_fail(CIMA_E_ARG, "attention_shared_tc: qkv rows must be 16-byte aligned");
   const CimaPaged pg{table, table_width, 0, page_size, nkv, hd, planes};
   const SharedArgs a{qkv, cache, pg, seq_slot, seq_len, order, own_page, groups, head_sink, slopes, part_o, part_ml, out,

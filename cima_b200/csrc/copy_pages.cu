@@ -85,7 +85,8 @@ extern "C" int cima_copy_pages(void* storage, int layers, long long pages, int s
   if (n <= 0) return 0;
   if (layers <= 0 || layers > 65535 || pages <= 0 || pages > 0x7fffffffll || segments <= 0 || page_size <= 0 || row_bytes <= 0)
     return cima_fail(CIMA_E_SIZE, "copy_pages: storage of %d layers, %lld pages, %d segments of %d positions of %lld bytes", layers, pages, segments, page_size, row_bytes);
-  if (row_bytes * page_size * segments >= (1ll << 31)) return cima_fail(CIMA_E_SIZE, "copy_pages: a page of %lld bytes; below 2^31 are possible", row_bytes * page_size * segments);
+  if (row_bytes >= (1ll << 30) || row_bytes * page_size >= (1ll << 30) || row_bytes * page_size * segments >= (1ll << 30))
+    return cima_fail(CIMA_E_SIZE, "copy_pages: pages of %d segments of %d positions of %lld bytes; below 2^30 bytes a page are possible", segments, page_size, row_bytes);
   const int width = (int)((unsigned long long)row_bytes | (unsigned long long)(uintptr_t)storage) & 15;
   const CopyPage* pg = reinterpret_cast<const CopyPage*>(plan);
   unsigned char* seen = (unsigned char*)calloc((size_t)pages, 1);       // 1: read, 2: written

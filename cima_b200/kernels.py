@@ -929,7 +929,7 @@ class Kernels:
         most = shared.most
         q = qkv.data_ptr()
         if tc is None:                                    # (the flag of the bounded waits lies on the device that first asked for it)
-            tc = (most * n_heads > SHARED_TC_ROWS * n_kv_heads and dtype is torch.bfloat16 and head_dim in (64, 128) and ld % 8 == 0 and q % 16 == 0
+            tc = (most * n_heads > SHARED_TC_ROWS * n_kv_heads and dtype is torch.bfloat16 and head_dim in (64, 128) and ld % 8 == 0 and q % 16 == 0 and scale >= 0
                   and pages * planes * n_kv_heads * size < 2 ** 31 and self.error_flag(qkv.device).get_device() == at)
         elif tc and dtype is not torch.bfloat16:
             raise KernelError(f"attention_shared: {dtype} on tcgen05; it takes bfloat16")

@@ -74,7 +74,7 @@ def shared_reference(c, *, head_sink=None, sink=0.0, slopes=None, gate_col=0):
         k, v = (held[:, i].permute(1, 0, 2, 3).reshape(nkv, -1, hd)[:, :n].repeat_interleave(G, 0) for i in (0, c.planes - 1))
         q = qkv[b, :nh * hd].view(nh, 1, hd)
         s = (q * k).sum(2) * c.scale
-        size = (q.abs() * k.abs()).sum(2) * c.scale
+        size = (q.abs() * k.abs()).sum(2) * abs(c.scale)
         back = torch.arange(n - 1, -1, -1, dtype=torch.float64)
         if slopes is not None:
             bias = slopes.cpu().double()[:, None] * back

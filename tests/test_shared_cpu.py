@@ -32,7 +32,7 @@ def test_bad_plans_of_copies(lib, plan, word):
 
 @pytest.mark.parametrize("args, word", [
     (dict(layers=0), "storage"), (dict(pages=0), "storage"), (dict(row=0), "storage"),
-    (dict(row=1 << 28), "2\\^31"), (dict(layers=70000), "storage"),
+    (dict(row=1 << 28), "2\\^30"), (dict(row=1 << 62), "2\\^30"), (dict(layers=70000), "storage"),
 ])
 def test_bad_storages_of_copies(lib, args, word):
     a = dict(base=BASE, layers=2, pages=4, segments=2, page=16, row=64) | args
@@ -65,12 +65,12 @@ def test_bad_arguments_of_shared_attention(lib, args, word):
 @pytest.mark.parametrize("args, word", [
     (dict(planes=3), "planes"), (dict(page=32), "page size"), (dict(nh=5), "multiple"), (dict(groups=3), "groups"), (dict(ps=0), "splits"), (dict(scratch=None), "scratch"),
     (dict(gate=300), "gate"), (dict(cache=BASE + 8), "aligned"), (dict(hd=96), "head_dim"), (dict(ld=516), "aligned"), (dict(pages=0), "pages"),
-    (dict(pages=1 << 24), "pages"), (dict(flag=None), "error flag"),
+    (dict(pages=1 << 24), "pages"), (dict(flag=None), "error flag"), (dict(scale=-0.125), "negative"), (dict(scale=float("nan")), "negative"),
 ])
 def test_bad_arguments_of_shared_attention_on_tcgen05(lib, args, word):
-    a = dict(ld=512, cache=BASE, pages=9, page=64, planes=2, groups=1, most=2, scratch=BASE, ps=2, os=2, nh=4, nkv=2, hd=64, gate=0, flag=BASE) | args
+    a = dict(ld=512, cache=BASE, pages=9, page=64, planes=2, groups=1, most=2, scratch=BASE, ps=2, os=2, nh=4, nkv=2, hd=64, gate=0, flag=BASE, scale=0.125) | args
     code = lib.cima_attention_shared_tc(BASE, a["ld"], a["cache"], a["pages"], BASE, 8, a["page"], a["planes"], BASE, BASE, BASE, BASE, BASE, a["groups"], a["most"],
-                                        a["scratch"], BASE, a["ps"], a["os"], BASE, 256, 2, a["nh"], a["nkv"], a["hd"], 0.125, 0.0, None, a["gate"], None, 0,
+                                        a["scratch"], BASE, a["ps"], a["os"], BASE, 256, 2, a["nh"], a["nkv"], a["hd"], a["scale"], 0.0, None, a["gate"], None, 0,
                                         a["flag"], None)
     assert code < 0
     assert word in lib.cima_last_error().decode()

@@ -127,6 +127,25 @@ def test_shared_attention_large_scores(K):
     check(run_shared(K, c), *shared_reference(c))
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("counts", [[3], [7], [40]])
+def test_shared_attention_of_rows_at_odd_places(K, counts, hd):
+    """Rows that begin 4 bytes behind a 16-byte boundary take the kernels that ask for no more."""
+    c = shared_case(counts, [3], [1, 64, 90], 4, 1, hd, torch.bfloat16, alone=[70], seed=4)
+    buf = torch.empty(c.qkv.numel() + 8, dtype=torch.bfloat16, device="cuda")
+    moved = buf[2:2 + c.qkv.numel()].view_as(c.qkv)
+    moved.copy_(c.qkv)
+    c.qkv = moved
+    check(run_shared(K, c), *shared_reference(c))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_shared_attention_of_a_negative_scale(K, dtype):
+    c = shared_case([12], [4], [1, 64, 90], 14, 2, 64, dtype, alone=[70], seed=4)
+    c.scale = -c.scale
+    check(run_shared(K, c), *shared_reference(c))
+
+
 def test_padded_groups_and_their_order(K):
     """Groups without sequences (a recorded step's spare places) take no part; the result does not depend on which spare places there are."""
     c = shared_case([3, 4], [2, 3], [1, 65], 14, 2, 64, torch.bfloat16, seed=5)
@@ -226,6 +245,18 @@ def test_copy_pages_of_a_large_storage(K):
     assert (x[1, 1198, :, :, :33] == 5).all() and (x[1, 1198, :, :, 33:] == 0).all() and (x[1, 0] == 5).all() and (x[0] == 0).all() and (x[1, 1:1198] == 0).all()
 
 
+def test_copy_pages_of_storage_at_odd_places(K):
+    """Storage that begins 2, 4 or 8 bytes behind a 16-byte boundary is moved in narrower pieces."""
+    shape = (2, 6, 2, 2, 16, 24)
+    for skip in (1, 2, 4):
+        buf = torch.randn(2 * 6 * 2 * 2 * 16 * 24 + 8, device="cuda").to(torch.bfloat16)
+        x = buf[skip:skip + 2 * 6 * 2 * 2 * 16 * 24].view(shape)
+        want, rest = x.clone(), buf[skip + x.numel():].clone()
+        want[:, 4, :, :, :7], want[:, 1] = x[:, 0, :, :, :7], x[:, 3]
+        K.copy_pages(x, torch.tensor([[0, 4, 7], [3, 1, 16]], dtype=torch.int32))
+        assert torch.equal(x, want) and torch.equal(buf[skip + x.numel():], rest)
+
+
 def test_copy_pages_replayed(K):
     x = torch.randn(2, 8, 2, 2, PAGE, 16, device="cuda")
     plan = torch.tensor([[0, 5, 20], [1, 6, 64]], dtype=torch.int32)
@@ -252,7 +283,7 @@ def test_copy_pages_refusals(K):
 
 
 # ---------------------------------------------------------------------------------------------- log-probabilities
-@pytest.mark.parametrize("n, V", [(1, 1), (1, 2), (3, 7), (1, 512), (5, 1000), (2, 4097), (64, 32003), (1, 151936), (61, 152064), (700, 5001), (66000, 5)])
+@pytest.mark.parametrize("n, V", [(1, 1), (1, 2), (3, 7), (1, 512), (5, 1000), (2, 4097), (64, 32003), (1, 151936), (61, 152064), (130, 40000), (700, 5001), (66000, 5), (66000, 1100)])
 @pytest.mark.parametrize("spread", [0.0, 3.0, 80.0])
 def test_token_logprobs(K, n, V, spread):
     gen = torch.Generator(device="cuda").manual_seed(n + V)
@@ -264,6 +295,40 @@ def test_token_logprobs(K, n, V, spread):
     want, tol = logprob_reference(x, t)
     off = (out.double() - want).abs()
     assert (off <= tol).all(), float((off / tol).max())
+
+
+@pytest.mark.parametrize("V", [1023, 1025, 4099, 151937])
+def test_token_logprobs_of_rows_at_odd_places(K, V):
+    """Rows that begin at any multiple of 4 bytes, and what lies beside them."""
+    for skip in (1, 2, 3):
+        buf = torch.full((5 * V + 8,), 1e30, device="cuda")
+        x = buf[skip:skip + 5 * V].view(5, V)
+        x.copy_(torch.randn(5, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(V + skip)))
+        t = torch.tensor([0, V - 1, 1, V // 2, V - 2], dtype=torch.int32, device="cuda")
+        out = torch.full((5,), 9.0, device="cuda")
+        K.token_logprobs(x, t, out)
+        want, tol = logprob_reference(x, t)
+        assert ((out.double() - want).abs() <= tol).all()
+
+
+def test_token_logprobs_replayed_and_on_a_stream(K):
+    x = torch.randn(9, 30000, device="cuda")
+    t = torch.randint(0, 30000, (9,), dtype=torch.int32, device="cuda")
+    want = torch.empty(9, device="cuda")
+    K.token_logprobs(x, t, want)
+    out, side = torch.empty(9, device="cuda"), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K.token_logprobs(x, t, out)
+    side.synchronize()
+    assert torch.equal(out, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        K.token_logprobs(x, t, out)
+    x.mul_(0.5)
+    g.replay()
+    K.token_logprobs(x, t, want)
+    assert torch.equal(out, want)
 
 
 def test_token_logprobs_of_infinite_logits(K):
