@@ -127,6 +127,46 @@ def test_shared_attention_large_scores(K):
     check(run_shared(K, c), *shared_reference(c))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("hd", [48, 64, 96, 128])
+@pytest.mark.parametrize("splits", [None, (1, 1), (2, 2), (3, 4), (2, 120)])
+def test_shared_attention_begun_early(K, splits, hd, dtype):
+    """A launch that reads its pages ahead of the kernel before it, which may still write each sequence's newest position: at the end of a page, at
+    its beginning, alone in the sequence; in the last of its own pages' splits or the only one."""
+    for counts in ([3], [40]):
+        c = shared_case(counts, [5], [1, 64, 65, 128, 300, 640], 8, 2, hd, dtype, alone=[1, 64, 65, 500], gate=True, seed=hd)
+        check(run_shared(K, c, splits=splits, early=True, gate_col=c.gate_col, slopes=c.slopes), *shared_reference(c, gate_col=c.gate_col, slopes=c.slopes))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_shared_attention_behind_the_write_of_its_newest_position(K, hd, dtype):
+    """The kernel that turns and stores a step's new keys, then at once the attention that begins early, many times over: what it reads is new."""
+    for counts, splits in ([3], None), ([40], None), ([40], (3, 4)):
+        c = shared_case(counts, [5], [1, 64, 65, 200], 8, 2, hd, dtype, alone=[64, 130], seed=hd)
+        first = run_shared(K, c, splits=splits)
+        cols = slice(0, c.heads * hd)
+        pages = c.table[c.slot.long(), (c.len.long() - 1) // PAGE].long()
+        at = (c.len.long() - 1) % PAGE
+        now = c.storage[pages, :, :, at].clone()
+        wrong, q = torch.full_like(now, 50.0), c.qkv[:, cols].clone()
+        g = torch.cuda.CUDAGraph()
+        got = torch.empty_like(first)
+        run = lambda: got.copy_(run_shared(K, c, splits=splits, early=True))     # noqa: E731
+        run()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            c.storage[pages, :, :, at] = wrong
+            c.qkv[:, cols] = 3.0
+            c.storage[pages, :, :, at] = now
+            c.qkv[:, cols] = q
+            run()
+        for _ in range(20):
+            g.replay()
+            assert torch.equal(got, first)
+        check(got, *shared_reference(c))
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("counts", [[3], [7], [40]])
 def test_shared_attention_of_rows_at_odd_places(K, counts, hd):
