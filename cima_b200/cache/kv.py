@@ -70,7 +70,7 @@ class LayerKV:
 
 @dataclass
 class SharedPrefixes:
-    """Which sequences of a step hold the same pages for a prefix, as an attention kernel wants it (int32 on the device; ``KVCache.shared_prefixes``
+    """Which sequences of a step hold the same pages for a prefix, as an attention kernel wants it (int32 on the device; ``KVCache.shared_groups``
     finds them).  The pages of a group are the first ones of all its sequences' tables and lie below their newest positions."""
     order: torch.Tensor          # [seqs] the step's sequences, group by group, those of no group at any place
     own_page: torch.Tensor       # [seqs] pages that sequence i has in common with its group (0: it is in none); its own begin there

@@ -926,6 +926,8 @@ class Kernels:
         n_groups, three = groups.shape
         if three != 3 or ld < width:
             raise KernelError(f"attention_shared: groups {tuple(groups.shape)} are not [groups, 3], or rows of {ld} hold no {n_heads} heads of {head_dim}")
+        if B == 0:
+            return
         most = shared.most
         q = qkv.data_ptr()
         if tc is None:                                    # (the flag of the bounded waits lies on the device that first asked for it)

@@ -186,6 +186,12 @@ def test_shared_attention_of_a_negative_scale(K, dtype):
     check(run_shared(K, c), *shared_reference(c))
 
 
+def test_shared_attention_of_no_sequences(K):
+    c = shared_case([3], [5], [1, 64], 8, 2, 64, torch.bfloat16)
+    c.qkv, c.B = c.qkv[:0], 0
+    assert run_shared(K, c).shape == (0, 512)
+
+
 def test_padded_groups_and_their_order(K):
     """Groups without sequences (a recorded step's spare places) take no part; the result does not depend on which spare places there are."""
     c = shared_case([3, 4], [2, 3], [1, 65], 14, 2, 64, torch.bfloat16, seed=5)
