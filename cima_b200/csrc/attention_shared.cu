@@ -11,6 +11,9 @@
 // tiles; 32: two, whose warps share a page's 64 keys).  Up to 16 rows, and a sequence's own pages, whose rows are the heads of its kv head, take
 // keys and values straight to registers (head sizes 64 and 128).  The parts go to scratch and k_shared_combine joins them in a fixed order.
 //
+// Bound: for the few rows that come here the chain of one block, plan, table, pages, merge.  Measured: 2 sequences over 320 positions, 14 heads on 2 of
+// 64 dims, 6.7 us with the merge; in float32 4 over 960 11.8 us, 54 over 7,360 104 us (its 1.4 GFLOP of multiply-adds would take 20 at 72 TFLOP/s).
+//
 // Scores, maxima, exponentials and sums are float32, base 2; probabilities are rounded to bfloat16 only as operand of P V.
 #include "attention_shared.cuh"
 

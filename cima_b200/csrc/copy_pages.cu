@@ -9,7 +9,8 @@
 // written: the copies of a plan have no order among them).
 //
 // Bound: bytes.  A thread moves four vectors of 16 bytes (narrower ones where a position's bytes or the storage are not so aligned), all
-// four on their way before the first is written.
+// four on their way before the first is written.  Measured: 333 pages of 28 layers (1.22 GB read and written) 186 us, 6.6 TB/s; 66 pages of 24 layers
+// (208 MB) 33 us, 6.3 TB/s; a page of 21 positions 1.5 us, 7 of 37 positions in 28 layers 3.9 us, which is the launch and latency of one load and store.
 #include "common.cuh"
 #include <stdlib.h>
 #include <string.h>

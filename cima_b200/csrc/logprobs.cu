@@ -2,6 +2,9 @@
 // by which finished continuations are ranked and given tokens scored.  One pass over the row with a running maximum and sum (float32), each thread its
 // own; threads, warps and the blocks of a cluster that share a row are joined in a fixed order.
 //
+// Bound: the bytes of the logits.  Measured, rows of 152,064: 2,000 177 us (6.9 TB/s, a part of them in L2), 61 9.4 us (3.9 TB/s: a cluster's
+// placement and meeting, and one round of loads a block), one 3.7 us, of which the launch and the cluster are most.
+//
 // As of the formula: a row with a NaN or with +inf, and a row of nothing but -inf, have no log-probabilities (NaN); a token of logit -inf has
 // -inf in any other row.  A token id outside the vocabulary gives NaN.
 #include "common.cuh"
