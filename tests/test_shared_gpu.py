@@ -186,6 +186,23 @@ def test_shared_attention_of_a_negative_scale(K, dtype):
     check(run_shared(K, c), *shared_reference(c))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("early", [False, True])
+@pytest.mark.parametrize("counts", [[3], [40]])
+def test_shared_attention_of_an_empty_sequence(K, counts, early, hd, dtype):
+    """A sequence without a position gives zeros, and the others what they gave."""
+    c = shared_case(counts, [5], [1, 64, 200], 8, 2, hd, dtype, alone=[64, 70, 1], gate=True, seed=hd)
+    more = dict(early=early, gate_col=c.gate_col, slopes=c.slopes, splits=(3, 2))
+    want = run_shared(K, c, **more)
+    empty = int((c.own_page == 0).nonzero()[1])
+    c.len[empty] = 0
+    got = run_shared(K, c, **more)
+    assert (got[empty] == 0).all()
+    keep = torch.arange(c.B, device="cuda") != empty
+    assert torch.equal(got[keep], want[keep])
+
+
 def test_shared_attention_of_no_sequences(K):
     c = shared_case([3], [5], [1, 64], 8, 2, 64, torch.bfloat16)
     c.qkv, c.B = c.qkv[:0], 0
