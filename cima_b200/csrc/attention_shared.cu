@@ -233,7 +233,7 @@ extern "C" int cima_attention_shared(const void* qkv, int dtype, int ld, const v
   if (B <= 0) return 0;
   const CimaPaged pg{table, table_width, 0, page_size, nkv, hd, planes};
   const SharedArgs a{qkv, cache, pg, seq_slot, seq_len, order, own_page, groups, head_sink, slopes, part_o, part_ml, out,
-                     ld, ldo, B, nh, nkv, n_groups, 0, prefix_splits, 0, own_splits, gate_col, early, scale, sink, 1, 16};
+                     ld, ldo, B, nh, nkv, n_groups, 0, prefix_splits, 0, own_splits, gate_col, early, scale, sink, 1, 16, 0};
   if (const int rc = check_shared("attention_shared", a, most)) return rc;
   if (dtype == CIMA_F32) {
     if (hd % 4 || hd < 4 || hd > 128) return cima_fail(CIMA_E_SIZE, "attention_shared: head_dim %d; in float32 this kernel takes multiples of 4 up to 128", hd);

@@ -66,6 +66,7 @@ struct SharedArgs {
   float scale, sink;
   int least;                      // pages of a split
   int own_rows;                   // rows of a block of a sequence's own pages
+  int prefix_first;               // order of the two sorts of blocks (is_prefix)
 };
 
 // The splits of `pages` pages, n at most and of at least `least` pages each (a split costs its results' way through memory and a place in the
@@ -86,15 +87,20 @@ struct Task {
 };
 
 __host__ __device__ __forceinline__ int own_blocks_of(const SharedArgs& a) { return a.B * a.nkv * a.own_tiles * a.own_splits; }
+__host__ __device__ __forceinline__ int prefix_blocks_of(const SharedArgs& a) { return a.n_groups * a.prefix_tiles * a.nkv * a.prefix_splits; }
 
-// The sequences' own pages first: they are the shorter ones, and the prefixes' blocks take their places as they end.  (In turn, one of each sort on
-// an SM, 64 sequences over 16,384 positions took 39 us instead of 35: a prefix's block walks no faster beside one that waits for memory than beside
-// its like.)  i: the block's index, then its index among its sort.
+// Which sort of blocks comes first; the other's take their places as they end.  On tcgen05 the prefixes where every sequence may be in a group (a
+// prefix's block has the longer chain), else the sequences' own pages, as one that shares nothing has the longest blocks.  Measured, prefixes first
+// against own pages first: 48 sequences over 1,664 positions, 40 heads on 8, 18.9 / 23.6 us; 8 groups of 22 over 256, 14.9 / 16.5; 64 over 16,384
+// with up to 500 of their own 42.4 / 42.0; 28 over 3,520 with up to 760 14.1 / 13.3; with sequences alone 36 and 2 over 11,584 48 / 41, 24 and 7 over
+// 1,536 15.0 / 13.2; in the step of 7B heads, us a layer, 64 over 2,048 4.7 less, 32 over 4,096 3.8, 16 over 8,192 3.4, 64 over 16,384 2.1.  (In turn,
+// one of each sort on an SM, 64 sequences over 16,384 positions took 39 us instead of 35: a prefix's block walks no faster beside one that waits for
+// memory than beside its like.)  i: the block's index, then its index among its sort.
 __device__ __forceinline__ bool is_prefix(const SharedArgs& a, int& i) {
-  const int own = own_blocks_of(a);
-  if (i < own) return false;
-  i -= own;
-  return true;
+  const int first = a.prefix_first ? prefix_blocks_of(a) : own_blocks_of(a);
+  if (i < first) return a.prefix_first;
+  i -= first;
+  return !a.prefix_first;
 }
 
 __device__ __forceinline__ bool find_task(const SharedArgs& a, int prefix_rows, Task& t) {
@@ -644,7 +650,7 @@ k_shared_combine(const __grid_constant__ SharedArgs a, int hd) {
   }
 }
 
-inline int blocks_of(const SharedArgs& a) { return a.n_groups * a.prefix_tiles * a.nkv * a.prefix_splits + own_blocks_of(a); }
+inline int blocks_of(const SharedArgs& a) { return prefix_blocks_of(a) + own_blocks_of(a); }
 
 template <int HD, int NB, int NW> __host__ __device__ constexpr size_t near_smem() { return (size_t)NW * 8 * NB * (HD + 3) * 4 + 8; }
 

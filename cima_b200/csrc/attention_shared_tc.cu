@@ -476,7 +476,7 @@ extern "C" int cima_attention_shared_tc(const void* qkv, int ld, const void* cac
   if (ld % 8 || ((uintptr_t)qkv & 15)) return cima_fail(CIMA_E_ARG, "attention_shared_tc: qkv rows must be 16-byte aligned");
   const CimaPaged pg{table, table_width, 0, page_size, nkv, hd, planes};
   const SharedArgs a{qkv, cache, pg, seq_slot, seq_len, order, own_page, groups, head_sink, slopes, part_o, part_ml, out,
-                     ld, ldo, B, nh, nkv, n_groups, 0, prefix_splits, 0, own_splits, gate_col, early, scale, sink, 2, 16};
+                     ld, ldo, B, nh, nkv, n_groups, 0, prefix_splits, 0, own_splits, gate_col, early, scale, sink, 2, 16, (long long)n_groups * most >= B};
   if (const int rc = check_shared("attention_shared_tc", a, most)) return rc;
   if (n_pages <= 0 || n_pages * planes * nkv * PS >= (1ll << 31)) return cima_fail(CIMA_E_SIZE, "attention_shared_tc: %lld pages exceed a tensor map's 32-bit row coordinate", n_pages);
   if (hd == 64) return planes == 2 ? launch_shared_tc<64, 2>(a, n_pages, most, error_flag, stream) : launch_shared_tc<64, 1>(a, n_pages, most, error_flag, stream);
