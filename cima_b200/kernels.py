@@ -119,6 +119,10 @@ def extend_splits(blocks: int, max_len: int, window: int, keep_first: int) -> in
 
 
 SHARED_TC_ROWS = 16         # query rows a kv head of the largest group, above which prefixes run on tcgen05 (blocks of 128 rows)
+# Blocks of prefixes on tcgen05, of the 296 that the SMs hold: the others' places are for the sequences' own pages meanwhile.  Measured with at most
+# 296 / 240 / 208 / 192 / 176 blocks, us (7B heads, sequences over positions, own ones up to): 64 over 16,384, 500 42.1 / 40.5 / 37.5 / 37.5 / 39.2; 37 over
+# 10,368, 771 33.2 / 31.8 / 29.5 / 28.0 / 26.4; 4 groups of 3 over 5,376, 27 20.3 / 17.2 / 17.7 / 17.9 / 18.6; over 101 drawn cases 0.7, 0.9, 0.9, 0.9 % shorter.
+SHARED_TC_BLOCKS = 200
 
 
 @lru_cache(maxsize=4096)
@@ -126,7 +130,7 @@ def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_head
     """(splits of a group's prefix, splits of a sequence's own pages) of ``Kernels.attention_shared``; the kernel leaves those without work that would have
     less than two pages (on tcgen05; else one), but a block without work still has to be placed.  ``rows``: query rows of a block of a prefix, 128 on
     tcgen05; ``prefix_pages``: a bound on a group's pages (0: none known).  Prefixes on tcgen05: some 96 blocks, for up to 8 sequences no more (one an SM then),
-    beyond them as many of four pages as one wave of two an SM holds.  Own pages, of which there mostly are few: some 64 blocks, at least one a sequence
+    beyond them as many of four pages as ``SHARED_TC_BLOCKS`` allows.  Own pages, of which there mostly are few: some 64 blocks, at least one a sequence
     and kv head; where sequences share nothing (there are more than the groups can hold) theirs are as long as the longest, and a block should have about 8
     of them, in four waves at most."""
     group, pages = n_heads // n_kv_heads, (max_len + 63) // 64 if max_len > 0 else 1 << 16
@@ -141,7 +145,7 @@ def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_head
         return max(1, min(96, 2 * SPLIT_BLOCKS // prefix, shared)), max(1, min(32, max(own, SPLIT_BLOCKS // blocks), pages))
     some = min(shared // least, 96 // prefix)
     if n_seqs > 8 or rows != 128:
-        some = max(some, min(shared // 4, SPLIT_BLOCKS // prefix))
+        some = max(some, min(shared // 4, (SHARED_TC_BLOCKS if rows == 128 else SPLIT_BLOCKS) // prefix))
     return max(1, min(48, some)), max(1, min(own, pages // least))
 
 
