@@ -9,11 +9,10 @@
 // leaves probabilities below 2^8.  The sequences' own pages are blocks of mma.sync as there, in the same launch: they are bound by bytes while the
 // prefixes are bound by the tensor cores.
 //
-// Measured, 28 heads on 4 of 128 dims, 64 sequences over 16,384 positions and up to 500 of their own (15 GFLOP, 67 MB): 37.4 us with the merge, of
-// which the prefixes' products are 13 at 925 cycles a page and 128 rows an SM (78 % of what a library product reaches), the own pages 8, the
-// chains before a block's first product and behind its last 5, the merge 5; 8 sequences over 2,048 10.7 us, a chain of latencies.  (A kernel of the
-// own pages alone beside one of the prefixes, a third launch, took 42.5, and 24 instead of 18.5 us where a few sequences share nothing: it was shorter,
-// by 10 to 25 %, only where own pages are few and many, 8 groups of 44 over 256 positions 19 instead of 26 us.)
+// Measured, 28 heads on 4 of 128 dims, 64 sequences over 16,384 positions and up to 500 of their own (15 GFLOP, 67 MB): 37.4 us with the merge.  A
+// prefix's block: 4.8 until its first product, 21 pages at 1,875 cycles (two blocks an SM: 925 a page of 128 rows, 78 % of what a library product
+// reaches), 2 to leave; own pages beside them; the merge 4.  8 sequences over 2,048 10.6 us, a chain of latencies.  (A kernel of the own pages alone
+// beside one of the prefixes, a third launch, was no shorter, and 24 instead of 18.5 us where a few sequences share nothing.)
 //
 // Every wait on an mbarrier is bounded (2 s); one that runs out sets *error_flag, and all roles leave their loops, free the tensor memory and
 // return.
