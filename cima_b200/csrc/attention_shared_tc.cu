@@ -6,12 +6,15 @@
 // thread (rows are gathered into the swizzled Q tile by them, then softmax); warp 4: TMA of K and V through the block table; warp 5: TMEM and the
 // MMAs.  S has two buffers, so S of the next page is computed while this one's probabilities are.  The K and V rings are two pages deep each.  Every key of a whole page is visible: no
 // mask.  The reference point of the exponentials moves when a row's maximum has grown by more than 2^8, which spares O most rescalings and
-// leaves probabilities below 2^8.  The sequences' own pages are blocks of mma.sync as there, in the same launch: they are bound by bytes while the
+// leaves probabilities below 2^8.  A probability goes into its product in two parts, its upper 16 bits and the next 8 of what they leave (2^-14 of it at most
+// is lost), over the two halves of its S: rounded to bfloat16 once, a row stood 2.2 to 2.35e-3 from 64 bits where the ordinary kernel, whose probabilities
+// are rounded against their own 16 keys' maximum, stands at 1.95e-3; in two parts 1.69e-3, the result's own rounding (the reference point at the maximum
+// and the rounded ones summed: 2.15e-3).  The second product costs 64 sequences over 16,384 positions 37.4 -> 45 us, 4 groups of 6 over 4,032 18.5 -> 20.7, 8 over
+// 2,048 nothing; the parts are cut off and not rounded, as two conversions a pair took 6 us more.  (An infinite value makes its column NaN.)  The sequences' own pages are blocks of mma.sync as there, in the same launch: they are bound by bytes while the
 // prefixes are bound by the tensor cores.
 //
-// Measured, 28 heads on 4 of 128 dims, 64 sequences over 16,384 positions and up to 500 of their own (15 GFLOP, 67 MB): 37.4 us with the merge.  A
-// prefix's block: 4.8 until its first product, 21 pages at 1,875 cycles (two blocks an SM: 925 a page of 128 rows, 78 % of what a library product
-// reaches), 2 to leave; own pages beside them; the merge 4.  8 sequences over 2,048 10.6 us, a chain of latencies.  (A kernel of the own pages alone
+// Measured, 28 heads on 4 of 128 dims, 64 sequences over 16,384 positions and up to 500 of their own (15 GFLOP, 67 MB): 45 us with the merge.  A
+// prefix's block: 4.8 until its first product, 21 pages at some 2,500 cycles (two blocks an SM; 1,875 with one product of P V a page), 2 to leave; own pages beside them; the merge 4.  8 sequences over 2,048 10.6 us, a chain of latencies.  (A kernel of the own pages alone
 // beside one of the prefixes, a third launch, was no shorter, and 24 instead of 18.5 us where a few sequences share nothing.)
 //
 // Every wait on an mbarrier is bounded (2 s); one that runs out sets *error_flag, and all roles leave their loops, free the tensor memory and
@@ -132,8 +135,8 @@ __device__ __forceinline__ void prefix_tc(const CUtensorMap* map, const SharedAr
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const unsigned long long vd = umma_smem_desc_mn(smem_u32(sv + (size_t)NH * s * KV_BLOCK), KV_BLOCK);
 #pragma unroll
-        for (int k = 0; k < PS / UMMA_K; k++)
-          umma_bf16_ts(tm_o, tm_s[s] + (unsigned)(k * (UMMA_K / 2)), vd + (unsigned long long)(k * (UMMA_K * 128 >> 4)), idesc_o, (j | k) ? 1u : 0u);
+        for (int k = 0; k < 2 * (PS / UMMA_K); k++)             // P in two parts, both against the same values
+          umma_bf16_ts(tm_o, tm_s[s] + (unsigned)(k * (UMMA_K / 2)), vd + (unsigned long long)(k % (PS / UMMA_K) * (UMMA_K * 128 >> 4)), idesc_o, (j | k) ? 1u : 0u);
         umma_commit(&v_empty[s]);
         umma_commit(pv_done);
       }
@@ -198,14 +201,16 @@ __device__ __forceinline__ void prefix_tc(const CUtensorMap* map, const SharedAr
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
       l_run *= alpha;
       float ps4[4] = {0.f, 0.f, 0.f, 0.f};
-      unsigned pk[32];
+      unsigned pk[32], rest[32];
 #pragma unroll
       for (int c = 0; c < 2; c++)
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float p0 = ex2(fmaf(__uint_as_float(raw[c][e]), sc2, neg_m));
           const float p1 = ex2(fmaf(__uint_as_float(raw[c][e + 1]), sc2, neg_m));
-          pk[c * 16 + (e >> 1)] = pack_bf16(p0, p1);
+          const unsigned u0 = __float_as_uint(p0), u1 = __float_as_uint(p1);
+          pk[c * 16 + (e >> 1)] = __byte_perm(u0, u1, 0x7632);
+          rest[c * 16 + (e >> 1)] = __byte_perm(__float_as_uint(p0 - __uint_as_float(u0 & 0xffff0000u)), __float_as_uint(p1 - __uint_as_float(u1 & 0xffff0000u)), 0x7632);
           ps4[(e >> 1) & 3] += p0 + p1;
         }
       l_run += (ps4[0] + ps4[1]) + (ps4[2] + ps4[3]);
@@ -222,7 +227,8 @@ __device__ __forceinline__ void prefix_tc(const CUtensorMap* map, const SharedAr
           tmem_st32(tm_o + lane_off + (unsigned)(c * 32), o);
         }
       }
-      tmem_st32_words(tm_s[s] + lane_off, pk);                 // P over the first 32 columns of its S
+      tmem_st32_words(tm_s[s] + lane_off, pk);                 // P over the first 32 columns of its S, what its rounding left over the others
+      tmem_st32_words(tm_s[s] + lane_off + 32u, rest);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[s]);                  // (one barrier a buffer: no waiter can be a phase behind)
