@@ -608,7 +608,9 @@ k_shared_combine(const __grid_constant__ SharedArgs a, int hd) {
   if (!a.early) wait_then_let_next();
   const int own = a.own_page[b];
   const int np = live_splits(own, a.prefix_splits, a.least), nr = live_splits(pages_of(a.seq_len[b]) - own, a.own_splits, a.least);
-  const float extra = a.head_sink ? expf(a.head_sink[h]) : a.sink;
+  // the entry without a value, as one more part: its score (base 2; a stored one of +inf stands for the largest number, against which all else is nothing)
+  // and how many of it there are.  (exp of the sink and of the maximum apart pass float32's range where their difference does not.)
+  const float sink_m = a.head_sink ? a.head_sink[h] * LOG2E : 0.f, extra_m = sink_m > 3e38f ? 3e38f : sink_m, extra_n = a.head_sink ? 1.f : a.sink;
   if (a.early) wait_then_let_next();
   float w[MAX_PARTS / 32], l[MAX_PARTS / 32], M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -620,6 +622,7 @@ k_shared_combine(const __grid_constant__ SharedArgs a, int hd) {
     M = fmaxf(M, ml.x);
   }
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if (extra_n != 0.f) M = fmaxf(M, extra_m);
   const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
   for (int i = 0; i < MAX_PARTS / 32; i++) {
@@ -627,8 +630,8 @@ k_shared_combine(const __grid_constant__ SharedArgs a, int hd) {
     L += w[i] * l[i];
   }
   for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  if (extra != 0.f) L += extra * exp2f(-ref);
-  const float inv = L > 0.f ? 1.0f / L : 0.f;
+  if (extra_n != 0.f) L += extra_n * exp2f(extra_m - ref);
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
   const int n = np + nr, d = 4 * lane;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = warp; s0 < n; s0 += 4 * COMBINE_WARPS) {
