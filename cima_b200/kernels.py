@@ -942,15 +942,17 @@ class Kernels:
         np_, no = splits or shared_splits(n_groups, most, B, n_heads, n_kv_heads, max_len, 128 if tc else 32 if dtype is torch.float32 else 16,
                                            shared.pages)
         if self.profile is not None and not self._admit(f"attention_shared[{np_} + {no} splits]", *self._attention_work(qkv, n_heads, n_kv_heads, head_dim, planes)): return
-        # this call's own, as attention_decode's
+        flag = self.error_flag(qkv.device) if tc else None
+        if tc:
+            self._here(flag)
+        # this call's own, as attention_decode's: held until the launch, or another thread's tensor, or the flag above, could be given the same memory
         cells = B * n_heads * (np_ + no)
-        part = qkv.new_empty(cells * (head_dim + 2), dtype=torch.float32).data_ptr()
+        scratch = qkv.new_empty(cells * (head_dim + 2), dtype=torch.float32)
+        part = scratch.data_ptr()
         rest = (table.data_ptr(), table.shape[1], size, planes, seq_slot.data_ptr(), seq_len.data_ptr(), order.data_ptr(), own_page.data_ptr(), groups.data_ptr(),
                 n_groups, most, part, part + 4 * cells * head_dim, np_, no, out.data_ptr(), width, B, n_heads, n_kv_heads, head_dim, scale, sink,
                 None if head_sink is None else head_sink.data_ptr(), gate_col, None if slopes is None else slopes.data_ptr(), 1 if early else 0)
         if tc:
-            flag = self.error_flag(qkv.device)
-            self._here(flag)
             self._check(self.lib.cima_attention_shared_tc(q, ld, storage.data_ptr(), pages, *rest, flag.data_ptr(), _raw_stream(at)), "attention_shared_tc")
         else:
             self._check(self.lib.cima_attention_shared(q, F32 if dtype is torch.float32 else dtype_code(dtype), ld, storage.data_ptr(), *rest, _raw_stream(at)),
