@@ -75,7 +75,7 @@ class LM:
         (temperature, top_k, top_p, repeat_penalty, seed, max_tokens, stop, ignore_eos), either as a
         ``GenOptions`` (one for all prompts or one per prompt) or as keyword arguments.  ``on_token(i, token)`` is
         called for every token of prompt ``i`` as soon as its step is read.
-        ``continuations`` n: n answers to each prompt, drawn with seeds that follow the option's (the first is what one answer would be); result and
+        ``continuations`` n: n answers to each prompt, each with a generator of its own that follows from the seed (the first is what one answer would be); result and
         request ``i * n + k`` is the k-th of prompt ``i``.  A prompt runs once for all its answers, which share its part of the cache.
         ``logprobs``: each result holds its tokens' log-probabilities (``logprobs``, ``logprob``) under the model's own distribution."""
         if named:

@@ -35,7 +35,7 @@ Usage:
        --stream                           print every token as its step is read ("<prompt>:<token>" a line)
        --dtype bfloat16|float32           precision of the whole model (default bfloat16)
        --max-seq N                        positions the cache holds in all (default 8192)
-       --continuations N                  N answers to each prompt, one a line, drawn with seeds that follow --seed (the prompt runs once)
+       --continuations N                  N answers to each prompt, one a line, drawn by generators that follow from --seed (the prompt runs once)
        --logprobs                         behind each answer, after a tab, the log-probability of its tokens together
        --PARAM VALUE                      generation parameters (see `cima run --help`)
   cima bench <MODEL_DIR> [-n TOKENS] [--iters N] [--batch B] [--prompt-len P]

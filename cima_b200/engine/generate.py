@@ -88,9 +88,10 @@ def fit_prompt(prompt: Sequence[int], max_position: int):
 
 
 def continuation(options: GenOptions, k: int) -> GenOptions:
-    """The options of a prompt's k-th continuation (from 0): the generator's seed k further on (0, which a generator takes as 1, is left
-    out), so that the first is what a single answer would be and no two draw alike."""
-    return options if k == 0 else replace(options, seed=(max(options.seed, 1) - 1 + k) % ((1 << 64) - 1) + 1)
+    """The options of a prompt's k-th continuation (from 0): the seed k further on (0, which a generator takes as 1, is left out), and marked as
+    the k-th answer, whose generator starts from both mixed (``GenOptions.generator_state``), so that its draws are apart from the others'; the first is what a
+    single answer would be."""
+    return options if k == 0 else replace(options, seed=(max(options.seed, 1) - 1 + k) % ((1 << 64) - 1) + 1, answer=options.answer + k)
 
 
 def plan_batches(needs: Sequence[int], max_batch: int, cache_tokens: int, page_size: int, shared: Optional[Sequence[int]] = None) -> List[List[int]]:
@@ -128,7 +129,7 @@ class GenerationLoop:
         """``on_token(i, token)`` is called for every token of request ``i`` as soon as the step that made it is
         read, in the order of the requests within a step (the reference hands each token's text to its
         ``on_token`` as it is generated, src/models/mod.rs:977, :1307); a stop token is not reported.
-        ``continuations`` n > 1: n answers to each prompt (request i n + k is the k-th of prompt i, drawn with ``continuation``'s seed), whose prompt
+        ``continuations`` n > 1: n answers to each prompt (request i n + k is the k-th of prompt i, drawn with ``continuation``'s options), whose prompt
         runs once.  ``logprobs``: the results hold their tokens' log-probabilities."""
         st = self.stepper
         self._on_token = on_token

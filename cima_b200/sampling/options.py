@@ -30,6 +30,16 @@ OPTION_TABLE = [
 ]
 
 
+_MASK, _GAMMA = (1 << 64) - 1, 0x9E3779B97F4A7C15      # (2^64 over the golden ratio)
+
+
+def _mixed(z: int) -> int:
+    z = (z + _GAMMA) & _MASK
+    z = (z ^ z >> 30) * 0xBF58476D1CE4E5B9 & _MASK
+    z = (z ^ z >> 27) * 0x94D049BB133111EB & _MASK
+    return z ^ z >> 31
+
+
 @dataclass(frozen=True)
 class GenOptions:
     temperature: float = 0.8
@@ -40,6 +50,15 @@ class GenOptions:
     max_tokens: int = 1024
     stop: tuple = ()
     ignore_eos: bool = False
+    answer: int = 0                   # which of several answers to one prompt this is (``engine.generate.continuation``); 0: a request of its own
+
+    @property
+    def generator_state(self) -> int:
+        """The state (of 64 bits, not 0) that the request's generator starts from: the seed itself, as the reference's; for a further answer seed and
+        answer mixed by the finalizer of SplitMix64 (Steele, Lea and Flood, 2014).  The generator is a shift register, whose first draws from
+        neighbouring states are neighbours: unmixed, answers drawn from the same logits would begin alike."""
+        state = max(int(self.seed), 1) & _MASK
+        return state if self.answer == 0 else max(_mixed(_mixed(state) + self.answer * _GAMMA), 1)
 
     @property
     def greedy(self) -> bool:

@@ -15,7 +15,6 @@ from ..cache.kv import StateRequest
 from .options import GenOptions
 
 RING = 64
-_MASK = (1 << 64) - 1
 
 
 def sampler_state() -> List[StateRequest]:
@@ -43,8 +42,7 @@ class DeviceSampler:
         ring = np.zeros((n, RING), dtype=np.int32)
         count = np.zeros((n, 1), dtype=np.int32)
         for i, (p, o) in enumerate(zip(prompts, options)):
-            state = max(int(o.seed), 1) & _MASK
-            rng[i, 0] = np.array(state, dtype=np.uint64).astype(np.int64)
+            rng[i, 0] = np.array(o.generator_state, dtype=np.uint64).astype(np.int64)
             tail = list(p)[-RING:]
             # the ring is indexed by (tokens pushed so far) % 64
             total = len(p)
