@@ -77,7 +77,8 @@ class LM:
         called for every token of prompt ``i`` as soon as its step is read.
         ``continuations`` n: n answers to each prompt, each with a generator of its own that follows from the seed (the first is what one answer would be); result and
         request ``i * n + k`` is the k-th of prompt ``i``.  A prompt runs once for all its answers, which share its part of the cache.
-        ``logprobs``: each result holds its tokens' log-probabilities (``logprobs``, ``logprob``) under the model's own distribution."""
+        ``logprobs``: each result holds its tokens' log-probabilities (``logprobs``; ``stop_logprob`` of a stop token that ended it) and their sum (``logprob``)
+        under the model's own distribution."""
         if named:
             if options is not None and not isinstance(options, GenOptions):
                 raise ValueError("keyword options go with at most one GenOptions")

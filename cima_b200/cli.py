@@ -36,7 +36,7 @@ Usage:
        --dtype bfloat16|float32           precision of the whole model (default bfloat16)
        --max-seq N                        positions the cache holds in all (default 8192)
        --continuations N                  N answers to each prompt, one a line, drawn by generators that follow from --seed (the prompt runs once)
-       --logprobs                         behind each answer, after a tab, the log-probability of its tokens together
+       --logprobs                         behind each answer, after a tab, its log-probability (its tokens and the stop token that ended it)
        --PARAM VALUE                      generation parameters (see `cima run --help`)
   cima bench <MODEL_DIR> [-n TOKENS] [--iters N] [--batch B] [--prompt-len P]
                                         Greedy decode rate, stop tokens ignored, one discarded warm-up

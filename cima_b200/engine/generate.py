@@ -33,11 +33,12 @@ class GenResult:
     prompt_tokens: int
     truncated: bool = False
     logprobs: Optional[List[float]] = None     # where asked for: of each token, under the model's own distribution (no penalty, temperature or cut)
+    stop_logprob: Optional[float] = None       # the same of the stop token that ended the answer and is not among its tokens
 
     @property
     def logprob(self) -> Optional[float]:
-        """Log-probability of the answer's tokens together (None where none were asked for)."""
-        return None if self.logprobs is None else sum(self.logprobs)
+        """Log-probability of the whole answer, its tokens and the stop token that ended it (None where none were asked for)."""
+        return None if self.logprobs is None else sum(self.logprobs) + (self.stop_logprob or 0.0)
 
 
 @dataclass
@@ -221,7 +222,7 @@ class GenerationLoop:
                 for j, t, score in zip(live, tokens, scores):
                     i = ids[j]
                     if t in stops[j] and not opts[i].ignore_eos:
-                        results[i] = GenResult(out[j], "stop", len(prompts[j]), fitted[i][1], lps[j] if logprobs else None)
+                        results[i] = GenResult(out[j], "stop", len(prompts[j]), fitted[i][1], lps[j] if logprobs else None, score)
                         continue
                     out[j].append(int(t))
                     if logprobs:

@@ -57,3 +57,29 @@ def test_the_sampler_starts_from_them():
     lm.stepper.sampler.begin([0, 1, 2], [[1], [2], [3]], options)
     got = [int(x) & (1 << 64) - 1 for x in lm.model.cache.state["sampler.rng"][:3, 0]]
     assert got == [o.generator_state for o in options] and got[0] == 9
+
+
+def _score(prompt, tokens):
+    cfg, W = plain_load(model_folder("B"))
+    whole = prompt + tokens
+    lp = torch.log_softmax(plain_forward(W, cfg, whole).double(), 1)
+    return [float(lp[k - 1, whole[k]]) for k in range(len(prompt), len(whole))]
+
+
+@pytest.mark.parametrize("after", [0, 1, 3])
+def test_an_answer_that_stops_is_scored_with_its_stop_token(after):
+    """Its log-probability is that of its tokens and the stop token, which it does not hold; one that stops at once is scored by that alone."""
+    lm, p = _lm("B"), random_tokens(TINY["B"]["vocab_size"], 20, 1)
+    opts = dict(max_tokens=6, temperature=0, repeat_penalty=1.0, logprobs=True)
+    (free,) = lm.generate([p], ignore_eos=True, **opts)
+    stop = free.tokens[after]
+    want = _score(p, free.tokens[:after + 1])
+    assert stop not in free.tokens[:after]
+    for n in (1, 3):
+        for r in lm.generate([p], stop=stop, continuations=n, **opts):
+            assert r.finish_reason == "stop" and r.tokens == free.tokens[:after]
+            assert r.logprobs == pytest.approx(want[:-1], abs=1e-3) and r.stop_logprob == pytest.approx(want[-1], abs=1e-3)
+            assert r.logprob == pytest.approx(sum(want), abs=5e-3) and r.logprob < 0
+    assert free.finish_reason == "length" and free.stop_logprob is None and free.logprob == pytest.approx(sum(free.logprobs))
+    (r,) = lm.generate([p], stop=stop, max_tokens=6, temperature=0, repeat_penalty=1.0)
+    assert r.finish_reason == "stop" and r.logprobs is None and r.stop_logprob is None and r.logprob is None
