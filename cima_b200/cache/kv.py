@@ -125,8 +125,8 @@ class KVGroup:
         return min(n, self.ring_pages) if self.ring_pages else n
 
     def written(self, slot: int, start: int, length: int) -> List[int]:
-        """Places among the slot's pages that positions start .. length - 1 lie in and that other slots hold too."""
-        if not self.shared:
+        """Places among the slot's pages that positions start .. length - 1 lie in (none where there are none) and that other slots hold too."""
+        if not self.shared or start >= length:
             return []
         held = self.pages_of[slot]
         return [i for i in range(start // self.page_size, min(len(held), -(-length // self.page_size))) if self.holders[held[i]] > 1]
