@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("pipeline", [True, False])
-@pytest.mark.parametrize("after", [0, 1, 4])
+@pytest.mark.parametrize("after", [0, 1, 3])
 def test_an_answer_that_stops_is_scored_with_its_stop_token(pipeline, after, always):
     lm = lm_of("tiny-b", "float32", pipeline=pipeline)
     p = tokens(1000, 140, 1)
