@@ -25,19 +25,45 @@ def test_two_threads(tc, streams):
 
     want = [call(c) for c in cases]
     torch.cuda.synchronize()
-    wrong, start = [0, 0], threading.Barrier(2)
+    wrong, start = [None, None], threading.Barrier(2)
 
     def work(i):
-        stream = torch.cuda.Stream() if streams == 2 else torch.cuda.current_stream()
-        start.wait(30)
-        with torch.cuda.stream(stream):
-            outs = [call(cases[i]) for _ in range(300)]
-            stream.synchronize()
-            wrong[i] = sum(not torch.equal(o, want[i]) for o in outs)
+        try:
+            stream = torch.cuda.Stream() if streams == 2 else torch.cuda.current_stream()
+            start.wait(30)
+            with torch.cuda.stream(stream):
+                outs = [call(cases[i]) for _ in range(300)]
+                stream.synchronize()
+                wrong[i] = sum(not torch.equal(o, want[i]) for o in outs)
+        except Exception as e:
+            wrong[i] = e
 
     threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
     for t in threads:
         t.start()
     for t in threads:
         t.join(60)
+    assert not any(isinstance(w, Exception) for w in wrong), wrong
     assert wrong == [0, 0] and K.device_errors() == 0
+
+
+def test_a_thread_without_a_context():
+    """A thread's first CUDA call may be a kernel that makes a tensor map."""
+    from cima_b200.kernels import Kernels
+    K = Kernels(verbose=False)
+    a, w = torch.randn(256, 128, device="cuda").bfloat16(), torch.randn(256, 128, device="cuda").bfloat16()
+    want, got = torch.empty(256, 256, dtype=torch.bfloat16, device="cuda"), torch.empty(256, 256, dtype=torch.bfloat16, device="cuda")
+    K.gemm_tc_pair(a, w, None, want, 0)
+    K.device_errors()
+    failed = []
+
+    def work():
+        try:
+            K.gemm_tc_pair(a, w, None, got, 0)
+        except Exception as e:
+            failed.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join(60)
+    assert not failed and torch.equal(got, want)
