@@ -77,6 +77,7 @@ class SharedPrefixes:
     groups: torch.Tensor         # [groups, 3] place of the group's first sequence in ``order``, sequences, pages
     most: int                    # sequences of the largest group
     pages: int = 0               # a bound on the pages of a group (0: not known), for the choice of splits only
+    alone: Optional[bool] = None # whether some sequence is in no group (None: where there are more than the groups could hold), for splits and order only
 
     @staticmethod
     def pack(groups: Sequence[Tuple[Sequence[int], int]], n_seqs: int) -> np.ndarray:
@@ -92,9 +93,9 @@ class SharedPrefixes:
         return out
 
     @classmethod
-    def over(cls, packed: torch.Tensor, n_seqs: int, most: int, pages: int = 0) -> "SharedPrefixes":
+    def over(cls, packed: torch.Tensor, n_seqs: int, most: int, pages: int = 0, alone: Optional[bool] = None) -> "SharedPrefixes":
         """The arrays of ``packed`` (on the device) as views."""
-        return cls(packed[:n_seqs], packed[n_seqs:2 * n_seqs], packed[2 * n_seqs:].view(-1, 3), most, pages)
+        return cls(packed[:n_seqs], packed[n_seqs:2 * n_seqs], packed[2 * n_seqs:].view(-1, 3), most, pages, alone)
 
 
 class KVGroup:

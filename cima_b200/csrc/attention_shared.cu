@@ -224,7 +224,7 @@ int launch_shared_f32(SharedArgs a, int hd, int most, cudaStream_t stream) {
 // Row b of qkv is sequence b's new position, which the cache holds already (as position seq_len[b] - 1).  order [B], own_page [B],
 // groups [n_groups, 3]: see SharedArgs; a group's pages are the same in all its sequences' tables and lie below their newest
 // positions; `most`: sequences of the largest group.  part_o / part_ml: scratch of B * nh * (prefix_splits + own_splits) * (hd, 2) floats.
-// early: as cima_attention_decode's.
+// early: as cima_attention_decode's (its lowest bit).
 extern "C" int cima_attention_shared(const void* qkv, int dtype, int ld, const void* cache, const int* table, int table_width, int page_size,
                                      int planes, const int* seq_slot, const int* seq_len, const int* order, const int* own_page, const int* groups,
                                      int n_groups, int most, float* part_o, float* part_ml, int prefix_splits, int own_splits, void* out, int ldo,
@@ -233,7 +233,7 @@ extern "C" int cima_attention_shared(const void* qkv, int dtype, int ld, const v
   if (B <= 0) return 0;
   const CimaPaged pg{table, table_width, 0, page_size, nkv, hd, planes};
   const SharedArgs a{qkv, cache, pg, seq_slot, seq_len, order, own_page, groups, head_sink, slopes, part_o, part_ml, out,
-                     ld, ldo, B, nh, nkv, n_groups, 0, prefix_splits, 0, own_splits, gate_col, early, scale, sink, 1, 16, 0};
+                     ld, ldo, B, nh, nkv, n_groups, 0, prefix_splits, 0, own_splits, gate_col, early & 1, scale, sink, 1, 16, 0};
   if (const int rc = check_shared("attention_shared", a, most)) return rc;
   if (dtype == CIMA_F32) {
     if (hd % 4 || hd < 4 || hd > 128) return cima_fail(CIMA_E_SIZE, "attention_shared: head_dim %d; in float32 this kernel takes multiples of 4 up to 128", hd);

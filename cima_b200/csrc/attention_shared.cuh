@@ -89,7 +89,7 @@ struct Task {
 __host__ __device__ __forceinline__ int own_blocks_of(const SharedArgs& a) { return a.B * a.nkv * a.own_tiles * a.own_splits; }
 __host__ __device__ __forceinline__ int prefix_blocks_of(const SharedArgs& a) { return a.n_groups * a.prefix_tiles * a.nkv * a.prefix_splits; }
 
-// Which sort of blocks comes first; the other's take their places as they end.  On tcgen05 the prefixes where every sequence may be in a group (a
+// Which sort of blocks comes first; the other's take their places as they end.  On tcgen05 the prefixes where every sequence is in a group (a
 // prefix's block has the longer chain), else the sequences' own pages, as one that shares nothing has the longest blocks.  Measured, prefixes first
 // against own pages first: 48 sequences over 1,664 positions, 40 heads on 8, 18.9 / 23.6 us; 8 groups of 22 over 256, 14.9 / 16.5; 64 over 16,384
 // with up to 500 of their own 42.4 / 42.0; 28 over 3,520 with up to 760 14.1 / 13.3; with sequences alone 36 and 2 over 11,584 48 / 41, 24 and 7 over

@@ -467,7 +467,8 @@ int launch_shared_tc(SharedArgs a, long long n_pages, int most, int* error_flag,
 
 }  // namespace
 
-// cima_attention_shared for bfloat16 and head sizes 64 and 128, blocks of 128 rows of a prefix on tcgen05.  n_pages: of the storage;
+// cima_attention_shared for bfloat16 and head sizes 64 and 128, blocks of 128 rows of a prefix on tcgen05.  early: 2 more where some sequence is in no
+// group (which sort of blocks comes first, is_prefix).  n_pages: of the storage;
 // error_flag: device int that a wait that ran out sets to 1 (never cleared here).
 extern "C" int cima_attention_shared_tc(const void* qkv, int ld, const void* cache, long long n_pages, const int* table, int table_width, int page_size,
                                         int planes, const int* seq_slot, const int* seq_len, const int* order, const int* own_page, const int* groups,
@@ -481,7 +482,7 @@ extern "C" int cima_attention_shared_tc(const void* qkv, int ld, const void* cac
   if (ld % 8 || ((uintptr_t)qkv & 15)) return cima_fail(CIMA_E_ARG, "attention_shared_tc: qkv rows must be 16-byte aligned");
   const CimaPaged pg{table, table_width, 0, page_size, nkv, hd, planes};
   const SharedArgs a{qkv, cache, pg, seq_slot, seq_len, order, own_page, groups, head_sink, slopes, part_o, part_ml, out,
-                     ld, ldo, B, nh, nkv, n_groups, 0, prefix_splits, 0, own_splits, gate_col, early, scale, sink, 2, 16, (long long)n_groups * most >= B};
+                     ld, ldo, B, nh, nkv, n_groups, 0, prefix_splits, 0, own_splits, gate_col, early & 1, scale, sink, 2, 16, !(early & 2)};
   if (const int rc = check_shared("attention_shared_tc", a, most)) return rc;
   if (n_pages <= 0 || n_pages * planes * nkv * PS >= (1ll << 31)) return cima_fail(CIMA_E_SIZE, "attention_shared_tc: %lld pages exceed a tensor map's 32-bit row coordinate", n_pages);
   if (hd == 64) return planes == 2 ? launch_shared_tc<64, 2>(a, n_pages, most, error_flag, stream) : launch_shared_tc<64, 1>(a, n_pages, most, error_flag, stream);

@@ -39,8 +39,14 @@ def shared_shape(groups) -> tuple:
     return (len(groups), max(len(members) for members, _ in groups), 1 << (max(pages for _, pages in groups) - 1).bit_length()) if groups else ()
 
 
+def step_shape(groups, n_seqs: int) -> tuple:
+    """``shared_shape`` of a step of ``n_seqs`` sequences, and whether some of them are in no group (the number of the groups and their largest do
+    not say so where groups are uneven); () where nothing is shared."""
+    return (*shared_shape(groups), sum(len(members) for members, _ in groups) < n_seqs) if groups else ()
+
+
 class SharedBuffer:
-    """The ``SharedPrefixes`` of a recorded step: arrays of fixed address, filled anew for other sequences of the same ``shared_shape``."""
+    """The ``SharedPrefixes`` of a recorded step: arrays of fixed address, filled anew for other sequences of the same ``step_shape``."""
 
     def __init__(self, shape: tuple, n_seqs: int, device):
         n = 2 * n_seqs + 3 * shape[0]
@@ -73,7 +79,7 @@ class DecodeGraph:
         takes; ``UNEVEN``: the same, of sequences far from one length).  A recorded step fixes its launches; one recorded for short
         or middling contexts takes the kernels' choices for them, and the stepper moves on to the next graph when a sequence outgrows the bound.  ``pool``: the memory that its
         recording shares with others (of the same caller: they run one after another, and nothing in it outlives a step).  ``shape``: the
-        ``shared_shape`` of sequences that share prefixes.  ``logprobs``: the chosen tokens' log-probabilities stand behind the tokens in ``result``."""
+        ``step_shape`` of sequences that share prefixes.  ``logprobs``: the chosen tokens' log-probabilities stand behind the tokens in ``result``."""
         self.model, self.sampler = model, sampler
         self.B = B = n_seqs
         self.all_greedy = all_greedy

@@ -25,7 +25,7 @@ from ..parts.linear import FOLDED_NORM_ROWS
 from ..parts.norm import RowsInfo
 from ..weights.loader import TensorSpec, tensor_names
 from .batch import StepBatch, StepEntry, build_batch, check_entries, lengths_are_even
-from .graph import UNEVEN, shared_shape
+from .graph import UNEVEN, step_shape
 from .fit import STEP_ROWS
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32,
@@ -297,13 +297,13 @@ class Model:
         groups = self.shared_groups([e.slot for e in entries]) if all(len(e.tokens) == 1 for e in entries) else []
         if record and self._recordable(entries):
             with self._step_lock:
-                g = self._step_graph([n + 1 for n in starts], shared_shape(groups))
+                g = self._step_graph([n + 1 for n in starts], step_shape(groups, len(entries)))
                 if g is not None:
                     return self._step_recorded(g, entries, starts, groups)
         batch = build_batch(entries, starts, self.spec.vocab, self.rt.device)
         if groups:
             packed = torch.from_numpy(SharedPrefixes.pack(groups, len(entries))).to(self.rt.device)
-            batch.shared = SharedPrefixes.over(packed, len(entries), *shared_shape(groups)[1:])
+            batch.shared = SharedPrefixes.over(packed, len(entries), *step_shape(groups, len(entries))[1:])
         for e, s in zip(entries, starts):
             cache.reserve(e.slot, s + len(e.tokens))
         cache.flush()

@@ -13,7 +13,7 @@ from ..cache.kv import CapacityError
 from ..sampling.options import GenOptions
 from ..sampling.sampler import DeviceSampler
 from .batch import StepEntry
-from .graph import MAX_PROMPT_GRAPHS, shared_shape
+from .graph import MAX_PROMPT_GRAPHS, step_shape
 
 
 MIN_REUSE = 16     # a finished sequence is taken up again only for at least this many tokens in common
@@ -369,7 +369,7 @@ class ModelStepper:
         bound = self._context_bound(slots, ahead)
         armed = self._armed[1:] if self._armed and self._armed[1] == tuple(slots) else None
         groups = armed[1] if armed else self.model.shared_groups(slots)      # (what is shared stays shared while these sequences go on)
-        key = (len(slots), all_greedy, bound, shared_shape(groups), self.logprobs)
+        key = (len(slots), all_greedy, bound, step_shape(groups, len(slots)), self.logprobs)
         graph = self._graphs.get(key)
         if graph is None:
             from .graph import DecodeGraph

@@ -126,20 +126,22 @@ SHARED_TC_BLOCKS = 200
 
 
 @lru_cache(maxsize=4096)
-def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_heads: int, max_len: int, rows: int = 128, prefix_pages: int = 0) -> Tuple[int, int]:
+def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_heads: int, max_len: int, rows: int = 128, prefix_pages: int = 0,
+                  alone: Optional[bool] = None) -> Tuple[int, int]:
     """(splits of a group's prefix, splits of a sequence's own pages) of ``Kernels.attention_shared``; the kernel leaves those without work that would have
     less than two pages (on tcgen05; else one), but a block without work still has to be placed.  ``rows``: query rows of a block of a prefix, 128 on
     tcgen05; ``prefix_pages``: a bound on a group's pages (0: none known).  Prefixes on tcgen05: some 96 blocks, for up to 8 sequences no more (one an SM then),
     beyond them as many of four pages as ``SHARED_TC_BLOCKS`` allows.  Own pages, of which there mostly are few: some 64 blocks, at least one a sequence
-    and kv head; where sequences share nothing (there are more than the groups can hold) theirs are as long as the longest, and a block should have about 8
-    of them, in four waves at most."""
+    and kv head; where sequences share nothing (``alone``; None: where there are more than the groups can hold) theirs are as long as the longest, and a block
+    should have about 8 of them, in four waves at most (one alone over 16,100 positions beside groups of 6 and 2 over 16,000, 7B heads: 40 us, 158 in one block a kv head; the
+    ordinary kernels 55)."""
     group, pages = n_heads // n_kv_heads, (max_len + 63) // 64 if max_len > 0 else 1 << 16
     prefix = max(1, n_groups * -(-most * group // rows) * n_kv_heads)
     blocks = n_seqs * n_kv_heads * -(-group // 16)
     shared = min(pages, prefix_pages) if prefix_pages else pages
     least = 2 if rows == 128 else 1
     own = min(4, 64 // blocks)
-    if n_seqs > n_groups * most:
+    if alone if alone is not None else n_seqs > n_groups * most:
         own = max(own, min(16, pages // 8, 4 * SPLIT_BLOCKS // blocks))
     if rows == 32:                                     # float32: a page is long work, and blocks are small
         return max(1, min(96, 2 * SPLIT_BLOCKS // prefix, shared)), max(1, min(32, max(own, SPLIT_BLOCKS // blocks), pages))
@@ -940,7 +942,7 @@ class Kernels:
         elif tc and dtype is not torch.bfloat16:
             raise KernelError(f"attention_shared: {dtype} on tcgen05; it takes bfloat16")
         np_, no = splits or shared_splits(n_groups, most, B, n_heads, n_kv_heads, max_len, 128 if tc else 32 if dtype is torch.float32 else 16,
-                                           shared.pages)
+                                           shared.pages, shared.alone)
         if self.profile is not None and not self._admit(f"attention_shared[{np_} + {no} splits]", *self._attention_work(qkv, n_heads, n_kv_heads, head_dim, planes)): return
         flag = self.error_flag(qkv.device) if tc else None
         if tc:
@@ -951,7 +953,8 @@ class Kernels:
         part = scratch.data_ptr()
         rest = (table.data_ptr(), table.shape[1], size, planes, seq_slot.data_ptr(), seq_len.data_ptr(), order.data_ptr(), own_page.data_ptr(), groups.data_ptr(),
                 n_groups, most, part, part + 4 * cells * head_dim, np_, no, out.data_ptr(), width, B, n_heads, n_kv_heads, head_dim, scale, sink,
-                None if head_sink is None else head_sink.data_ptr(), gate_col, None if slopes is None else slopes.data_ptr(), 1 if early else 0)
+                None if head_sink is None else head_sink.data_ptr(), gate_col, None if slopes is None else slopes.data_ptr(),
+                (1 if early else 0) + (2 if (shared.alone if shared.alone is not None else B > n_groups * most) else 0))
         if tc:
             self._check(self.lib.cima_attention_shared_tc(q, ld, storage.data_ptr(), pages, *rest, flag.data_ptr(), _raw_stream(at)), "attention_shared_tc")
         else:
