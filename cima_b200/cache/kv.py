@@ -80,10 +80,11 @@ class SharedPrefixes:
     alone: Optional[bool] = None # whether some sequence is in no group (None: where there are more than the groups could hold), for splits and order only
 
     @staticmethod
-    def pack(groups: Sequence[Tuple[Sequence[int], int]], n_seqs: int) -> np.ndarray:
-        """``KVCache.shared_groups``' answer for a step of ``n_seqs`` sequences as the three arrays one behind the other."""
+    def pack(groups: Sequence[Tuple[Sequence[int], int]], n_seqs: int, places: int = 0) -> np.ndarray:
+        """``KVCache.shared_groups``' answer for a step of ``n_seqs`` sequences as the three arrays one behind the other, with at least ``places`` groups (the
+        further ones have no sequences)."""
         order = [i for members, _ in groups for i in members]
-        out = np.zeros(2 * n_seqs + 3 * len(groups), dtype=np.int32)
+        out = np.zeros(2 * n_seqs + 3 * max(len(groups), places), dtype=np.int32)
         out[:n_seqs] = order + sorted(set(range(n_seqs)) - set(order))
         at = 0
         for k, (members, pages) in enumerate(groups):

@@ -40,9 +40,15 @@ def shared_shape(groups) -> tuple:
 
 
 def step_shape(groups, n_seqs: int) -> tuple:
-    """``shared_shape`` of a step of ``n_seqs`` sequences, and whether some of them are in no group (the number of the groups and their largest do
-    not say so where groups are uneven); () where nothing is shared."""
-    return (*shared_shape(groups), sum(len(members) for members, _ in groups) < n_seqs) if groups else ()
+    """What the attention of a one-token step of ``n_seqs`` sequences that share prefixes fixes of them, and so what its recordings are kept by:
+    ``shared_shape`` with groups and largest rounded up to powers of two (groups without sequences and rows without a sequence take no part), and whether some
+    of them are in no group (which the numbers do not say where groups are uneven); () where nothing is shared.  Answers that end one after another pass
+    through a shape a step: of 8 prompts of 4, of 31 in a later batch 3 are new with 64 kept, 11 by the exact numbers."""
+    if not groups:
+        return ()
+    n, most, pages = shared_shape(groups)
+    up = lambda v: 1 << (v - 1).bit_length()                  # noqa: E731
+    return min(up(n), max(n, n_seqs // 2)), min(up(most), n_seqs), pages, sum(len(members) for members, _ in groups) < n_seqs
 
 
 class SharedBuffer:
@@ -50,12 +56,12 @@ class SharedBuffer:
 
     def __init__(self, shape: tuple, n_seqs: int, device):
         n = 2 * n_seqs + 3 * shape[0]
-        self.n_seqs = n_seqs
+        self.n_seqs, self.places = n_seqs, shape[0]
         self.device = torch.zeros(n, dtype=torch.int32, device=device)
         self.shared = SharedPrefixes.over(self.device, n_seqs, *shape[1:])
 
     def load(self, groups) -> None:
-        host = torch.from_numpy(SharedPrefixes.pack(groups, self.n_seqs))
+        host = torch.from_numpy(SharedPrefixes.pack(groups, self.n_seqs, self.places))
         self.device.copy_(host.pin_memory() if self.device.is_cuda else host, non_blocking=True)
 
 
@@ -146,6 +152,7 @@ PROMPT_BUCKETS = (16, 32, 64, 128, 256, 384, 512, 768, 1024, 1536, 2048)    # ro
 PROMPT_ROWS = 256                           # rows (all sequences together) that every model's prompt steps are recorded for
 
 
+MAX_SHARED_GRAPHS = 128    # recorded decode steps of sequences that share prefixes kept (0.9 MB each of 28 layers); the one used longest ago gives way
 MAX_PROMPT_GRAPHS = 24    # recorded prompt steps kept (by sequences and rows); the one used longest ago gives way
 
 

@@ -302,8 +302,9 @@ class Model:
                     return self._step_recorded(g, entries, starts, groups)
         batch = build_batch(entries, starts, self.spec.vocab, self.rt.device)
         if groups:
-            packed = torch.from_numpy(SharedPrefixes.pack(groups, len(entries))).to(self.rt.device)
-            batch.shared = SharedPrefixes.over(packed, len(entries), *step_shape(groups, len(entries))[1:])
+            places, *shape = step_shape(groups, len(entries))
+            packed = torch.from_numpy(SharedPrefixes.pack(groups, len(entries), places)).to(self.rt.device)
+            batch.shared = SharedPrefixes.over(packed, len(entries), *shape)
         for e, s in zip(entries, starts):
             cache.reserve(e.slot, s + len(e.tokens))
         cache.flush()

@@ -13,6 +13,7 @@ from ..cache.kv import CapacityError
 from ..sampling.options import GenOptions
 from ..sampling.sampler import DeviceSampler
 from .batch import StepEntry
+from . import graph as recorded
 from .graph import MAX_PROMPT_GRAPHS, step_shape
 
 
@@ -370,10 +371,7 @@ class ModelStepper:
         armed = self._armed[1:] if self._armed and self._armed[1] == tuple(slots) else None
         groups = armed[1] if armed else self.model.shared_groups(slots)      # (what is shared stays shared while these sequences go on)
         key = (len(slots), all_greedy, bound, step_shape(groups, len(slots)), self.logprobs)
-        graph = self._graphs.get(key)
-        if graph is None:
-            from .graph import DecodeGraph
-            graph = self._graphs[key] = DecodeGraph(self.model, self.sampler, len(slots), all_greedy, bound, self._graph_pool, key[3], self.logprobs)
+        graph = self._graph(key)
         if self._armed is None or self._armed[:2] != (key, tuple(slots)):
             params = np.array([[o.temperature, float(o.top_k), o.top_p, o.repeat_penalty] for o in options], dtype=np.float32)
             carried = None
@@ -391,6 +389,23 @@ class ModelStepper:
         elif last_tokens is not None:
             graph.feed(last_tokens)
             self.h2d_bytes += 4 * len(slots)
+        return graph
+
+    def _graph(self, key):
+        """The recording of ``key`` (sequences, all greedy, context bound, ``step_shape``, log-probabilities), made where there is none.  Those of sequences
+        that share nothing are few and all kept; of the others, whose shapes follow how a batch's answers end, the ``MAX_SHARED_GRAPHS`` used last."""
+        graph = self._graphs.pop(key, None) if key[3] else self._graphs.get(key)
+        if graph is None:
+            if key[3]:
+                busy = [self._armed[0]] if self._armed else []
+                if self._flight is not None:
+                    busy += [k for k, g in self._graphs.items() if g is self._flight["graph"]]
+                old = [k for k in self._graphs if k[3] and k not in busy]
+                for k in old[:max(0, sum(1 for k in self._graphs if k[3]) + 1 - recorded.MAX_SHARED_GRAPHS)]:
+                    torch.cuda.synchronize()                # it may still be running
+                    del self._graphs[k]
+            graph = recorded.DecodeGraph(self.model, self.sampler, key[0], key[1], key[2], self._graph_pool, key[3], key[4])
+        self._graphs[key] = graph                           # (one of sequences that share: the last now)
         return graph
 
     def recorded_launches(self, n_seqs: int) -> int:

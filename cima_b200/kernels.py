@@ -136,7 +136,8 @@ def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_head
     should have about 8 of them, in four waves at most (one alone over 16,100 positions beside groups of 6 and 2 over 16,000, 7B heads: 40 us, 158 in one block a kv head; the
     ordinary kernels 55)."""
     group, pages = n_heads // n_kv_heads, (max_len + 63) // 64 if max_len > 0 else 1 << 16
-    prefix = max(1, n_groups * -(-most * group // rows) * n_kv_heads)
+    # (blocks with rows: uneven groups, and ones rounded up, have fewer than the numbers would give)
+    prefix = max(1, min(n_groups * -(-most * group // rows), n_groups + n_seqs * group // rows) * n_kv_heads)
     blocks = n_seqs * n_kv_heads * -(-group // 16)
     shared = min(pages, prefix_pages) if prefix_pages else pages
     least = 2 if rows == 128 else 1

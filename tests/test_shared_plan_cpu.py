@@ -14,10 +14,9 @@ def test_a_sequence_alone_beside_uneven_groups_is_not_taken_for_a_shared_one():
     they are beside even groups."""
     even, uneven = [([0, 1], 250), ([2, 3], 250)], [([0, 1, 2, 3, 4, 5], 250), ([6, 7], 250)]
     assert step_shape(even, 5) == (2, 2, 256, True) and step_shape(even, 4) == (2, 2, 256, False)
-    assert step_shape(uneven, 9) == (2, 6, 256, True) and step_shape(uneven, 8) == (2, 6, 256, False) and step_shape([], 8) == ()
-    assert step_shape(uneven, 9)[:3] == shared_shape(uneven)
+    assert step_shape(uneven, 9) == (2, 8, 256, True) and step_shape(uneven, 8) == (2, 8, 256, False) and step_shape([], 8) == ()
     for heads, kv, rows in ((28, 4, 128), (28, 4, 16), (40, 8, 128)):
-        own = [shared_splits(n, m, B, heads, kv, 16100, rows, 256, alone)[1] for n, m, B, alone in ((2, 2, 5, True), (2, 6, 9, True), (2, 6, 8, False))]
+        own = [shared_splits(n, m, B, heads, kv, 16100, rows, 256, alone)[1] for n, m, B, alone in ((2, 2, 5, True), (2, 8, 9, True), (2, 8, 8, False))]
         assert own[0] == own[1] >= 8 and own[2] < own[1]
     # not told, it goes by the numbers alone
     assert shared_splits(2, 2, 5, 28, 4, 16100) == shared_splits(2, 2, 5, 28, 4, 16100, alone=True)
@@ -41,4 +40,76 @@ def test_a_step_says_whether_some_sequence_is_alone(monkeypatch, extra):
     monkeypatch.setattr(lm.model, "forward", lambda batch: (seen.append(batch.shared), whole(batch))[1])
     lm.step([StepEntry(s, [1], [0]) for s in slots])
     (shared,) = seen
-    assert shared.alone == bool(extra) and shared.groups.tolist() == [[0, 3, 1], [3, 2, 1]] and shared.most == 3
+    assert shared.alone == bool(extra) and shared.groups.tolist() == [[0, 3, 1], [3, 2, 1]] and shared.most == 4
+
+
+def _endings(rng, prompts, answers):
+    """The plans that a batch of several prompts' answers passes through as they end one after another."""
+    left = [answers] * prompts
+    while any(left):
+        at, groups = 0, []
+        for n in left:
+            if n > 1:
+                groups.append((list(range(at, at + n)), 250))
+            at += n
+        yield groups, at
+        alive = [i for i, n in enumerate(left) if n]
+        left[rng.choice(alive)] -= 1
+
+
+def test_the_shapes_that_answers_pass_through_stay_few():
+    import random
+    rng = random.Random(1)
+    for prompts, answers in ((3, 8), (8, 4), (1, 32)):
+        seen, exact = {}, set()
+        for _ in range(300):
+            for groups, n in _endings(rng, prompts, answers):
+                shape = step_shape(groups, n)
+                if not groups:
+                    assert shape == ()
+                    continue
+                g, most, pages, alone = shape
+                assert len(groups) <= g <= n and max(len(m) for m, _ in groups) <= most <= n and pages == 256
+                assert alone == (sum(len(m) for m, _ in groups) < n)
+                seen.setdefault(n, set()).add(shape)
+                exact.add((n, *shared_shape(groups), alone))
+        total = sum(len(s) for s in seen.values())
+        assert total <= len(exact) and (prompts == 1) <= (total == answers - 1)
+        if prompts > 1:
+            assert total < 0.6 * len(exact)
+
+
+def test_spare_places_of_a_plan_are_groups_without_sequences():
+    from cima_b200.cache import SharedPrefixes
+    packed = SharedPrefixes.pack([([1, 3], 5)], 4, 3)
+    assert packed.tolist() == [1, 3, 0, 2] + [0, 5, 0, 5] + [0, 2, 5] + [0] * 6
+
+
+def test_recordings_of_sequences_that_share_are_bounded(monkeypatch):
+    """So many are kept, the one used longest ago gives way, but not what is armed or in flight; those of sequences that share nothing are kept all."""
+    from types import SimpleNamespace
+    import torch
+    from cima_b200.engine import graph
+    lm = _lm("B")
+    st = lm.stepper
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    monkeypatch.setattr(graph, "DecodeGraph", lambda model, sampler, n, greedy, bound, pool, shape, logprobs: SimpleNamespace(key=(n, greedy, bound, shape, logprobs)))
+    monkeypatch.setattr(graph, "MAX_SHARED_GRAPHS", 4)
+    key = lambda n, shape=(): (n, True, 0, shape, False)                # noqa: E731
+    shared = lambda n: key(n, (1, n, 4, False))                         # noqa: E731
+    plain = [st._graph(key(n)) for n in range(1, 40)]
+    first = st._graph(shared(2))
+    assert first.key == shared(2) and st._graph(shared(2)) is first
+    flown = st._graph(shared(3))
+    st._armed, st._flight = (shared(2), (), []), {"graph": flown}
+    for n in range(4, 20):
+        assert st._graph(shared(n)).key == shared(n)
+        kept = [k for k in st._graphs if k[3]]
+        assert len(kept) <= 4 and shared(2) in kept and shared(3) in kept and shared(n) in kept
+    assert [k for k in st._graphs if k[3]][-2:] == [shared(18), shared(19)]
+    st._armed = st._flight = None
+    st._graph(shared(18))
+    for n in range(20, 23):
+        st._graph(shared(n))
+    assert [k for k in st._graphs if k[3]] == [shared(18), shared(20), shared(21), shared(22)]
+    assert all(st._graphs[key(n)] is g for n, g in zip(range(1, 40), plain))
