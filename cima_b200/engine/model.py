@@ -89,6 +89,7 @@ class Model:
         self.config = None                                  # set by load_model
         self.step_rows = STEP_ROWS                          # a step of more rows runs in parts
         self.record_steps = False                           # record one-token steps (``StepGraph``); an ``LM`` with graphs says so
+        self._any_shared: Optional[bool] = None             # what ``_reads_shared`` found
         self._context_classes: Dict[int, tuple] = {}        # sequences -> what ``context_bound`` chooses among
         self._step_graphs = OrderedDict()                   # (sequences, context bound) -> StepGraph, the newest last
         self._step_pool = None                              # (memory pool, stream) that the recordings share
@@ -316,12 +317,21 @@ class Model:
     def shared_groups(self, slots: Sequence[int]):
         """What a one-token step of ``slots`` may read once for several of them (``KVCache.shared_groups``), where that is worth it."""
         cache = self.cache
-        groups = cache.shared_groups(slots)
+        groups = cache.shared_groups(slots) if self._reads_shared() else []
         if not groups:
             return []
         r = next(g.request for g in cache.groups if not g.ring_pages)
         page_bytes = r.planes * r.n_kv_heads * cache.page_size * r.head_dim * torch.empty((), dtype=cache.dtype).element_size()
         return groups if worth_sharing(groups, len(slots), page_bytes, self.rt.full_precision) else []
+
+    def _reads_shared(self) -> bool:
+        """Whether some layer's attention can read a common prefix once (a plan for none would only make recordings of its own)."""
+        if self.cache.page_size != 64:
+            return False
+        if self._any_shared is None:
+            mixers = [m for b in self.blocks for m in getattr(getattr(b, "mixer", None), "branches", [getattr(b, "mixer", None)])]
+            self._any_shared = any(getattr(m, "reads_shared", False) for m in mixers)
+        return self._any_shared
 
     def _recordable(self, entries: Sequence[StepEntry]) -> bool:
         """Whether the step runs through a ``StepGraph``: one token a sequence, every sequence's logits wanted, parts that may

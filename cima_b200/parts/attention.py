@@ -214,6 +214,11 @@ class Attention:
         from ..kernels import short_context
         return short_context(self.hd)
 
+    @property
+    def reads_shared(self) -> bool:
+        """Whether a one-token step may read a prefix that sequences have in common once (``Kernels.attention_shared``)."""
+        return not self.spec.window and self.hd <= 128
+
     def near_context(self, n_seqs: int, even: bool = True) -> Optional[int]:
         """Positions up to which the decode kernel of middling contexts takes a step of ``n_seqs`` sequences, of about one length (``even``)
         or not; 0: any number, None: it takes none."""

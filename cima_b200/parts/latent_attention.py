@@ -156,6 +156,11 @@ class LatentAttention:
     graph_safe = True
 
     @property
+    def reads_shared(self) -> bool:
+        """As ``Attention.reads_shared``."""
+        return not int(self.spec.window) and self.kd <= 128 and self.kd % (4 if self.rt.full_precision else 16) == 0
+
+    @property
     def short_context(self) -> int:
         from ..kernels import short_context
         return short_context(self.kd)

@@ -113,3 +113,25 @@ def test_recordings_of_sequences_that_share_are_bounded(monkeypatch):
         st._graph(shared(n))
     assert [k for k in st._graphs if k[3]] == [shared(18), shared(20), shared(21), shared(22)]
     assert all(st._graphs[key(n)] is g for n, g in zip(range(1, 40), plain))
+
+
+def test_no_plan_is_made_where_no_layer_could_read_it(monkeypatch):
+    """Head sizes above 128, windows, shared value heads and pages other than 64 take the ordinary kernels: no plan, and no recordings of their own."""
+    from cima_b200.parts.attention import Attention
+    from cima_b200.parts.diff_attention import DiffAttention
+    assert not getattr(DiffAttention, "reads_shared", False)
+    monkeypatch.setattr(engine_model, "worth_sharing", lambda groups, *a: bool(groups))
+
+    def groups(lm):
+        (a,) = lm.model.cache.open(1)
+        lm.step([StepEntry(a, random_tokens(TINY["B"]["vocab_size"], 70, 1))])
+        return lm.model.shared_groups([a] + lm.model.cache.fork(a, 2))
+
+    assert groups(_lm("B")) == [([0, 1, 2], 1)]
+    lm = _lm("B")
+    for block in lm.model.blocks:
+        assert isinstance(block.mixer, Attention) and block.mixer.reads_shared
+        block.mixer.hd = 144
+        assert not block.mixer.reads_shared
+    monkeypatch.setattr(Attention, "reads_shared", False)
+    assert groups(_lm("B")) == []
