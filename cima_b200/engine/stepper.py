@@ -384,7 +384,7 @@ class ModelStepper:
             graph.load(slots, last_tokens if carried is None else [0] * len(slots), [cache.length(s) for s in slots], params, groups)
             if carried is not None:
                 graph.tokens.copy_(carried)
-            self.h2d_bytes += 4 * (6 * len(slots) + 1) + params.nbytes
+            self.h2d_bytes += 4 * (6 * len(slots) + 1) + params.nbytes + (4 * graph.shared.device.numel() if graph.shared is not None else 0)
             self._armed = (key, tuple(slots), groups)
         elif last_tokens is not None:
             graph.feed(last_tokens)

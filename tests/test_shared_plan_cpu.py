@@ -135,3 +135,26 @@ def test_no_plan_is_made_where_no_layer_could_read_it(monkeypatch):
         assert not block.mixer.reads_shared
     monkeypatch.setattr(Attention, "reads_shared", False)
     assert groups(_lm("B")) == []
+
+
+def test_the_plan_counts_among_the_bytes_sent(monkeypatch):
+    """A recorded step's inputs as they are loaded: tokens, places, lengths and slots, the options, and the plan of what is shared."""
+    from types import SimpleNamespace
+    from cima_b200.engine import graph
+    from cima_b200.sampling import GenOptions
+    monkeypatch.setattr(engine_model, "worth_sharing", lambda groups, *a: bool(groups))
+    lm = _lm("B", max_tokens=2048)
+    st, c = lm.stepper, lm.model.cache
+    (a,) = c.open(1)
+    lm.step([StepEntry(a, random_tokens(TINY["B"]["vocab_size"], 70, 1))])
+    slots = [a] + c.fork(a, 2)
+
+    def recording(model, sampler, n, greedy, bound, pool, shape, logprobs):
+        shared = graph.SharedBuffer(shape, n, "cpu") if shape else None
+        return SimpleNamespace(load=lambda s, t, lengths, params, groups: shared and shared.load(groups), feed=lambda t: None, shared=shared, max_len=bound)
+
+    monkeypatch.setattr(graph, "DecodeGraph", recording)
+    for some, plan in ((slots, 2 * 3 + 3 * 1), (slots[:1], 0)):
+        before = st.h2d_bytes
+        st._arm(some, [1] * len(some), [GenOptions()] * len(some))
+        assert st.h2d_bytes - before == 4 * (6 * len(some) + 1 + 4 * len(some) + plan)
