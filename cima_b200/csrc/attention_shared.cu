@@ -189,6 +189,7 @@ int launch_shared_rows(SharedArgs a, int most, cudaStream_t stream) {
   a.own_rows = PRE > 0 ? rows : 16;
   a.own_tiles = (G + a.own_rows - 1) / a.own_rows;
   a.least = PRE > 0 ? 1 : 2;
+  a.own_least = own_least_of(a);
   constexpr size_t smem = PRE > 0 ? near_smem<HD, PRE, WARPS>() : walk_smem<HD, PLANES>();
   if (const int rc = prepare_kernel<k_attention_shared<HD, PLANES, RW, PRE>>(smem)) return rc;
   if (const int rc = cima_launch(k_attention_shared<HD, PLANES, RW, PRE>, dim3(blocks_of(a)), dim3(WARPS * 32), smem, stream, 1, a)) return rc;

@@ -67,6 +67,7 @@ struct SharedArgs {
   int least;                      // pages of a split
   int own_rows;                   // rows of a block of a sequence's own pages
   int prefix_first;               // order of the two sorts of blocks (is_prefix)
+  int own_least = 1;              // pages of a split of a sequence's own (own_least_of)
 };
 
 // The splits of `pages` pages, n at most and of at least `least` pages each (a split costs its results' way through memory and a place in the
@@ -85,6 +86,9 @@ struct Task {
   int kvh, rows, row0, G, group_first, seq, slot, first, last, part, len;
   bool prefix;
 };
+
+// Where there are blocks enough, a split of own pages only for 8 of them: a part more costs its way through memory and the merge, and most sequences have few.
+inline int own_least_of(const SharedArgs& a) { return (long long)a.B * a.nkv * a.own_tiles * a.own_splits > 64 ? 8 : a.least; }
 
 __host__ __device__ __forceinline__ int own_blocks_of(const SharedArgs& a) { return a.B * a.nkv * a.own_tiles * a.own_splits; }
 __host__ __device__ __forceinline__ int prefix_blocks_of(const SharedArgs& a) { return a.n_groups * a.prefix_tiles * a.nkv * a.prefix_splits; }
@@ -133,7 +137,7 @@ __device__ __forceinline__ bool find_task(const SharedArgs& a, int prefix_rows, 
     t.group_first = 0;
     const int from = a.own_page[t.seq];
     t.len = a.seq_len[t.seq];
-    const Share s = share_of(pages_of(t.len) - from, split, a.own_splits, a.least);
+    const Share s = share_of(pages_of(t.len) - from, split, a.own_splits, a.own_least);
     t.first = from + s.first, t.last = from + s.last, t.part = a.prefix_splits + split;
     if (s.first >= s.last) return false;
   }
@@ -607,7 +611,7 @@ k_shared_combine(const __grid_constant__ SharedArgs a, int hd) {
   const size_t base = (size_t)row * parts;
   if (!a.early) wait_then_let_next();
   const int own = a.own_page[b];
-  const int np = live_splits(own, a.prefix_splits, a.least), nr = live_splits(pages_of(a.seq_len[b]) - own, a.own_splits, a.least);
+  const int np = live_splits(own, a.prefix_splits, a.least), nr = live_splits(pages_of(a.seq_len[b]) - own, a.own_splits, a.own_least);
   // the entry without a value, as one more part: its score (base 2; a stored one of +inf stands for the largest number, against which all else is nothing)
   // and how many of it there are.  (exp of the sink and of the maximum apart pass float32's range where their difference does not.)
   const float sink_m = a.head_sink ? a.head_sink[h] * LOG2E : 0.f, extra_m = sink_m > 3e38f ? 3e38f : sink_m, extra_n = a.head_sink ? 1.f : a.sink;

@@ -450,6 +450,7 @@ int launch_shared_tc(SharedArgs a, long long n_pages, int most, int* error_flag,
   constexpr int WIDE = HD == 64 ? 2 : 1;                        // (16 rows are too many for the registers at head size 128: two blocks of 8)
   a.own_rows = 8 * (G <= 8 ? 1 : WIDE);
   a.own_tiles = (G + a.own_rows - 1) / a.own_rows;
+  a.own_least = own_least_of(a);
   constexpr size_t smem = tc_smem<HD>();
   static_assert(smem <= ONE_AN_SM && smem >= near_smem<HD, WIDE, 4>() && smem >= OWN_STAGES * 2 * (HD / 64) * KV_BLOCK + 16 * OWN_STAGES + 32, "a sequence's own pages and their merge fit");
   const dim3 grid(blocks_of(a));

@@ -132,7 +132,9 @@ def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_head
     less than two pages (on tcgen05; else one), but a block without work still has to be placed.  ``rows``: query rows of a block of a prefix, 128 on
     tcgen05; ``prefix_pages``: a bound on a group's pages (0: none known).  Prefixes on tcgen05: some 96 blocks, for up to 8 sequences no more (one an SM then),
     beyond them as many of four pages as ``SHARED_TC_BLOCKS`` allows.  Own pages, of which there mostly are few: some 64 blocks, at least one a sequence
-    and kv head; where sequences share nothing (``alone``; None: where there are more than the groups can hold) theirs are as long as the longest, and a block
+    and kv head, up to 8 sequences with places for as many blocks as the SMs hold where they may be long (the kernel uses one for every 8 pages: 8 over 6,144 positions with up to
+    8,192 of their own, 7B heads, 50 us; 62.5 with two a sequence and kv head, the ordinary kernels 52.  More sequences fill the SMs, and blocks without work cost 16 over 8,192
+    with few of their own 2 us); where sequences share nothing (``alone``; None: where there are more than the groups can hold) theirs are as long as the longest, and a block
     should have about 8 of them, in four waves at most (one alone over 16,100 positions beside groups of 6 and 2 over 16,000, 7B heads: 40 us, 158 in one block a kv head; the
     ordinary kernels 55)."""
     group, pages = n_heads // n_kv_heads, (max_len + 63) // 64 if max_len > 0 else 1 << 16
@@ -141,7 +143,7 @@ def shared_splits(n_groups: int, most: int, n_seqs: int, n_heads: int, n_kv_head
     blocks = n_seqs * n_kv_heads * -(-group // 16)
     shared = min(pages, prefix_pages) if prefix_pages else pages
     least = 2 if rows == 128 else 1
-    own = min(4, 64 // blocks)
+    own = max(min(4, 64 // blocks), min(8, SPLIT_BLOCKS // blocks, pages // 16) if n_seqs <= 8 else 0)
     if alone if alone is not None else n_seqs > n_groups * most:
         own = max(own, min(16, pages // 8, 4 * SPLIT_BLOCKS // blocks))
     if rows == 32:                                     # float32: a page is long work, and blocks are small

@@ -158,3 +158,11 @@ def test_the_plan_counts_among_the_bytes_sent(monkeypatch):
         before = st.h2d_bytes
         st._arm(some, [1] * len(some), [GenOptions()] * len(some))
         assert st.h2d_bytes - before == 4 * (6 * len(some) + 1 + 4 * len(some) + plan)
+
+
+def test_few_sequences_that_may_be_long_have_places_for_their_own_pages():
+    """Up to eight sequences over thousands of positions: blocks for long own parts, within what the SMs hold; short contexts and more sequences keep the few."""
+    own = lambda n, heads, kv, longest: shared_splits(1, n, n, heads, kv, longest, 128, 96)[1]                # noqa: E731
+    for n, heads, kv in ((8, 28, 4), (4, 28, 4), (8, 12, 2), (8, 40, 8)):
+        assert min(8, 296 // (n * kv)) == own(n, heads, kv, 14000) and n * kv * own(n, heads, kv, 14000) <= 296
+    assert own(8, 28, 4, 900) == 2 and own(16, 28, 4, 14000) == 1 and own(64, 28, 4, 30000) == 1
