@@ -471,23 +471,40 @@ class KVCache:
         full = [int(self.lengths[s]) // self.page_size for s in slots]
         rows = g.table_host[slots]
 
-        def split(members: List[int], depth: int):
-            if len(members) < 2:
-                return 0, []
+        # the tree of the prefixes, a node after the one that it is under (not by recursion: a sequence forked from the one before makes it as deep as
+        # there are sequences): members, pages common to them, nodes below
+        nodes: List[Tuple[List[int], int, List[int]]] = []
+        todo = [(list(range(len(slots))), 0, -1)]
+        while todo:
+            members, depth, above = todo.pop()
             most = min(full[i] for i in members)
             same = (rows[members, depth:most] == rows[members[0], depth:most]).all(0)
             common = depth + (int(same.argmin()) if not same.all() else most - depth)
+            if above >= 0:
+                nodes[above][2].append(len(nodes))
+            nodes.append((members, common, []))
             children: Dict[int, List[int]] = {}
             for i in members:
                 if full[i] > common:
                     children.setdefault(int(rows[i, common]), []).append(i)
-            parts = [split(c, common) for c in children.values()]
-            spared = sum(n for n, _ in parts)
-            if (len(members) - 1) * common >= spared:
-                return (len(members) - 1) * common, [(members, common)] if common else []
-            return spared, [p for _, ps in parts for p in ps]
-
-        return split(list(range(len(slots))), 0)[1]
+            todo += [(c, common, len(nodes) - 1) for c in reversed(list(children.values())) if len(c) > 1]
+        # from below: a node's own prefix, or the best of those under it, whichever spares more
+        spared = [0] * len(nodes)
+        whole = [False] * len(nodes)
+        for k in range(len(nodes) - 1, -1, -1):
+            members, common, below = nodes[k]
+            under = sum(spared[j] for j in below)
+            whole[k] = (len(members) - 1) * common >= under
+            spared[k] = max((len(members) - 1) * common, under)
+        out, look = [], [0]
+        while look:
+            k = look.pop()
+            members, common, below = nodes[k]
+            if not whole[k]:
+                look += reversed(below)
+            elif common:
+                out.append((members, common))
+        return out
 
     def trim(self, slot: int) -> int:
         """Give back the slot's pages behind those that its positions lie in (taken ahead, or left by a rewind); how many."""

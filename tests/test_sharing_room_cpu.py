@@ -63,3 +63,27 @@ def test_reserving_at_the_length_in_random_histories():
             c.reserve(slot, c.length(slot))
         assert [(g.pool.held, g.shared, list(g.copies)) for g in c.groups] == held
         s.verify()
+
+
+@pytest.mark.parametrize("n", [40, 1500])
+def test_groups_among_sequences_each_forked_from_the_one_before(n):
+    """Sequence i holds a page more than the one it was forked from: n prefixes one within the other, and in the comb two leaves at each."""
+    from cima_b200.cache import KVCache, KVRequest
+    c = KVCache([[KVRequest(1, 1, 0)]], 64 * 3 * n, 64 * (n + 2), __import__("torch").float32, "cpu")
+    (a,) = c.open(1)
+    chain = []
+    for _ in range(n):
+        c.reserve(a, c.length(a) + 64)
+        c.commit(a, c.length(a) + 64)
+        chain.append(a)
+        (a,) = c.fork(a)
+    # of prefix k (pages), n - k + 1 sequences: (n - k) k pages spared
+    (members, pages), = c.shared_groups(chain)
+    assert (len(members) - 1) * pages == max((n - k) * k for k in range(1, n)) and sorted(members) == list(range(pages - 1, n))
+    # two sequences that end at each length: pairs spare what the whole chain does, and more
+    pairs = chain + [c.fork(s)[0] for s in chain[:n // 2]]
+    got = c.shared_groups(pairs)
+    assert sum((len(m) - 1) * p for m, p in got) >= max((n - k) * k for k in range(1, n))
+    assert all(len(set(c.groups[0].table_host[pairs[i], p - 1] for i in m)) == 1 for m, p in got)
+    seen = [i for m, _ in got for i in m]
+    assert len(seen) == len(set(seen))
