@@ -12,7 +12,8 @@
 // keys and values straight to registers (head sizes 64 and 128).  The parts go to scratch and k_shared_combine joins them in a fixed order.
 //
 // Bound: for the few rows that come here the chain of one block, plan, table, pages, merge.  Measured: 2 sequences over 320 positions, 14 heads on 2 of
-// 64 dims, 6.7 us with the merge; in float32 4 over 960 11.8 us, 54 over 7,360 104 us (its 1.4 GFLOP of multiply-adds would take 20 at 72 TFLOP/s).
+// 64 dims, 6.6 us with the merge; 24 over 2,560, 8 heads on 2 of 96, 11.7; in float32 4 over 960 12.0 us, 54 over 7,360 72 us (its 1.4 GFLOP of multiply-adds would take
+// 20 at 72 TFLOP/s; a page is loaded, then multiplied).
 //
 // Scores, maxima, exponentials and sums are float32, base 2; probabilities are rounded to bfloat16 only as operand of P V.
 #include "attention_shared.cuh"

@@ -95,11 +95,10 @@ __host__ __device__ __forceinline__ int prefix_blocks_of(const SharedArgs& a) { 
 
 // Which sort of blocks comes first; the other's take their places as they end.  On tcgen05 the prefixes where every sequence is in a group (a
 // prefix's block has the longer chain), else the sequences' own pages, as one that shares nothing has the longest blocks.  Measured, prefixes first
-// against own pages first: 48 sequences over 1,664 positions, 40 heads on 8, 18.9 / 23.6 us; 8 groups of 22 over 256, 14.9 / 16.5; 64 over 16,384
-// with up to 500 of their own 42.4 / 42.0; 28 over 3,520 with up to 760 14.1 / 13.3; with sequences alone 36 and 2 over 11,584 48 / 41, 24 and 7 over
-// 1,536 15.0 / 13.2; in the step of 7B heads, us a layer, 64 over 2,048 4.7 less, 32 over 4,096 3.8, 16 over 8,192 3.4, 64 over 16,384 2.1.  (In turn,
-// one of each sort on an SM, 64 sequences over 16,384 positions took 39 us instead of 35: a prefix's block walks no faster beside one that waits for
-// memory than beside its like.)  i: the block's index, then its index among its sort.
+// against own pages first: 48 sequences over 1,664 positions, 40 heads on 8, 20.3 / 24.4 us; 8 groups of 22 over 256, 28 on 4, 27.1 / 32.4; 64 over 16,384
+// with up to 500 of their own 43.0 / 51.0; 28 over 3,520 with up to 760 20.3 / 19.5; with sequences alone 36 and 2 over 11,584 44.9 / 40.9, 24 and 7 over
+// 1,536 19.6 / 19.1; over 50 drawn cases the other order is 3 % longer.  (In turn, one of each sort on an SM, was 4 us longer for 64 over 16,384 when a page
+// was one product of P V: a prefix's block walks no faster beside one that waits for memory than beside its like.)  i: the block's index, then its index among its sort.
 __device__ __forceinline__ bool is_prefix(const SharedArgs& a, int& i) {
   const int first = a.prefix_first ? prefix_blocks_of(a) : own_blocks_of(a);
   if (i < first) return a.prefix_first;

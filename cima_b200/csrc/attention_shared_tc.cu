@@ -9,13 +9,13 @@
 // leaves probabilities below 2^8.  A probability goes into its product in two parts, its upper 16 bits and the next 8 of what they leave (2^-14 of it at most
 // is lost), over the two halves of its S: rounded to bfloat16 once, a row stood 2.2 to 2.35e-3 from 64 bits where the ordinary kernel, whose probabilities
 // are rounded against their own 16 keys' maximum, stands at 1.95e-3; in two parts 1.69e-3, the result's own rounding (the reference point at the maximum
-// and the rounded ones summed: 2.15e-3).  The second product costs 64 sequences over 16,384 positions 37.4 -> 45 us, 4 groups of 6 over 4,032 18.5 -> 20.7, 8 over
-// 2,048 nothing; the parts are cut off and not rounded, as two conversions a pair took 6 us more.  (An infinite value makes its column NaN.)  The sequences' own pages are blocks of mma.sync as there, in the same launch: they are bound by bytes while the
+// and the rounded ones summed: 2.15e-3).  The second product costs 64 sequences over 16,384 positions 37.4 -> 42.8 us, 4 groups of 6 over 4,032 18.5 -> 20.1, 8 over
+// 2,048 10.6 -> 11.7; the parts are cut off and not rounded, as two conversions a pair took 6 us more.  (An infinite value makes its column NaN.)  The sequences' own pages are blocks of mma.sync as there, in the same launch: they are bound by bytes while the
 // prefixes are bound by the tensor cores.
 //
-// Measured, 28 heads on 4 of 128 dims, 64 sequences over 16,384 positions and up to 500 of their own (15 GFLOP, 67 MB): 45 us with the merge.  A
-// prefix's block: 4.8 until its first product, 21 pages at some 2,500 cycles (two blocks an SM; 1,875 with one product of P V a page), 2 to leave; own pages beside them; the merge 4.  8 sequences over 2,048 10.6 us, a chain of latencies.  (A kernel of the own pages alone
-// beside one of the prefixes, a third launch, was no shorter, and 24 instead of 18.5 us where a few sequences share nothing.)
+// Measured, 28 heads on 4 of 128 dims, 64 sequences over 16,384 positions and up to 500 of their own (15 GFLOP, 67 MB): 42.8 us with the merge.  A
+// prefix's block: 4.8 until its first product, 21 pages at some 2,500 cycles (two blocks an SM; 1,875 with one product of P V a page), 2 to leave; own pages beside them; the merge 4.  8 sequences over 2,048 11.7 us, a chain of latencies.  (A kernel of the own pages alone
+// beside one of the prefixes, a third launch, was no shorter, and 5 us longer where a few sequences share nothing.)
 //
 // Every wait on an mbarrier is bounded (2 s); one that runs out sets *error_flag, and all roles leave their loops, free the tensor memory and
 // return.

@@ -41,9 +41,9 @@ def parse_dtype(d) -> torch.dtype:
 def worth_sharing(groups, n_seqs: int, page_bytes: int, full_precision: bool) -> bool:
     """Whether a one-token step's attention is the shorter for reading the groups' prefixes once: by the bytes that a layer is spared (``page_bytes``: of a page
     of one layer), which the ordinary kernels read again from L2 in about the time that this one takes beside them where they are 70 MB.  Measured in the
-    step, 7B heads, us a layer against the ordinary kernels (MB spared): 8 sequences over 2,048 / 8,192 / 16,384 positions +1.7 (29) / -3 (117) / -15
-    (235); 4 over 16,384 -10 (101); 16 over 2,048 / 8,192 -1.2 (63) / -21 (252); 32 over 1,024 / 2,048 +1.3 (65) / -5 (130); 48 over 448 / 1,000 / 2,048 0
-    (43) / -7 (92) / -22 (197); 64 over 640 0 (83).  In
+    step, 7B heads, us a layer against the ordinary kernels (MB spared): 8 sequences over 2,048 / 8,192 / 16,384 positions +3.4 (29) / -3 (117) / -14
+    (235); 4 over 16,384 -7 (101); 16 over 2,048 / 8,192 -0.5 (63) / -20 (252); 32 over 1,024 / 2,048 +1.7 (65) / -5 (130); 48 over 448 / 1,000 / 2,048 +1
+    (43) / -7 (92) / -20 (197); 64 over 640 0 (83).  In
     float32 (multiply-adds, one launch after another, 0.5B heads) 2 sequences over 64 / 256 6.7 / 8.9, 10.6 / 9.0 us ordinary / shared, 8 over 256 /
     1,024 10.7 / 15.2, 23.0 / 17.1, 16 over 1,024 33.2 / 18.8."""
     spared = page_bytes * sum((len(members) - 1) * pages for members, pages in groups)

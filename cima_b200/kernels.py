@@ -120,8 +120,8 @@ def extend_splits(blocks: int, max_len: int, window: int, keep_first: int) -> in
 
 SHARED_TC_ROWS = 16         # query rows a kv head of the largest group, above which prefixes run on tcgen05 (blocks of 128 rows)
 # Blocks of prefixes on tcgen05, of the 296 that the SMs hold: the others' places are for the sequences' own pages meanwhile.  Measured with at most
-# 296 / 240 / 208 / 192 / 176 blocks, us (7B heads, sequences over positions, own ones up to): 64 over 16,384, 500 42.1 / 40.5 / 37.5 / 37.5 / 39.2; 37 over
-# 10,368, 771 33.2 / 31.8 / 29.5 / 28.0 / 26.4; 4 groups of 3 over 5,376, 27 20.3 / 17.2 / 17.7 / 17.9 / 18.6; over 101 drawn cases 0.7, 0.9, 0.9, 0.9 % shorter.
+# 296 / 240 / 200 / 176 blocks, us (7B heads, sequences over positions, own ones up to): 64 over 16,384, 500 46.1 / 44.5 / 43.0 / 45.6; 37 over 10,368,
+# 771 36.0 / 35.3 / 30.2 / 29.2; 4 groups of 3 over 5,376, 27 22.2 / 19.3 / 20.3 / 21.2; over 50 cases 1.0 % longer, 0.2 % shorter, as it is, 0.5 % longer.
 SHARED_TC_BLOCKS = 200
 
 
