@@ -717,7 +717,7 @@ inline int check_shared(const char* who, const SharedArgs& a, int most) {
   if (a.gate_col < 0 || (a.gate_col > 0 && a.gate_col + a.nh * a.pg.head_dim > a.ld))
     return cima_fail(CIMA_E_ARG, "%s: %d gate values from column %d on exceed the rows of %d", who, a.nh * a.pg.head_dim, a.gate_col, a.ld);
   if ((uintptr_t)a.cache & 15) return cima_fail(CIMA_E_ARG, "%s: the cache must be 16-byte aligned", who);
-  const long long G = a.nh / a.nkv, blocks = ((long long)a.n_groups * ((most * G + 15) / 16) * a.prefix_splits + (long long)a.B * ((G + 7) / 8) * a.own_splits) * a.nkv;
+  const long long G = a.nh / a.nkv, blocks = ((long long)a.n_groups * ((most * G + 7) / 8) * a.prefix_splits + (long long)a.B * ((G + 7) / 8) * a.own_splits) * a.nkv;
   if (blocks > 0x7fffffffll || (long long)a.B * a.nh > 0x7fffffffll) return cima_fail(CIMA_E_SIZE, "%s: %lld blocks, or %d rows of %d heads, exceed one launch", who, blocks, a.B, a.nh);
   return 0;
 }
