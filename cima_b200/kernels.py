@@ -914,7 +914,7 @@ class Kernels:
                 and seq_slot.is_contiguous() and seq_len.is_contiguous() and order.is_contiguous() and own_page.is_contiguous() and groups.is_contiguous()
                 and qkv.get_device() == out.get_device() == storage.get_device() == table.get_device() == seq_slot.get_device() == seq_len.get_device()
                 == order.get_device() == own_page.get_device() == groups.get_device() == at
-                and qkv.dim() == 2 and storage.dim() == 5 and table.dim() == 2 and groups.dim() == 2):
+                and qkv.dim() == 2 and out.dim() == 2 and storage.dim() == 5 and table.dim() == 2 and groups.dim() == 2):
             self._need(qkv, "qkv", None, 2); self._need(out, "out", dtype, 2); self._need(storage, "cache", dtype, 5)
             for n, t, d in (("block_table", table, 2), ("seq_slot", seq_slot, 1), ("seq_len", seq_len, 1), ("order", order, 1), ("own_page", own_page, 1), ("groups", groups, 2)):
                 self._need(t, n, torch.int32, d)
